@@ -239,6 +239,76 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
                           int64_t* out_ids_dev, float* out_scores_dev, int32_t* out_counts_dev,
                           void* stream);
 
+/* ---- learned projections in front of a table (no counterpart in the reference, whose vectors arrive ready for
+ * the table: app.py:315-325, :384-391) -----------------------------------------------------------------------
+ * Rows that were embedded elsewhere are mapped into a table's space before they are inserted or searched with:
+ *   grouped   y_i = W[g] x_i                        one matrix for each source (encoder), rows grouped by source
+ *   adapted   y_i = W x_i + s[a] B[a] (A[a] x_i)    one matrix for all, a low-rank adapter for each request
+ * and both have their gradients, to fit the maps on relevance data.
+ *
+ * Segments.  Rows [n, dim] lie one after the other in segments (sources, requests): `offsets` is a device array of
+ * int64, one more than there are segments, that does not decrease; segment s holds rows
+ * [offsets[s], offsets[s + 1]).  Segments may be empty.  Rows outside every segment are left as they were in y and dx and
+ * take no part in the other gradients.  Offsets outside [0, n] are cut to it; where they decrease the
+ * results are undefined, but nothing outside the operands is read or written.
+ *
+ * Layout.  Weights are contiguous; rows may be `ld` elements apart, ld >= the row's length.  An output may share no
+ * element with an input.  Any sizes and any alignment to the element are taken; rows, matrices and leading
+ * dimensions that are multiples of 16 bytes are the fast ones.
+ *
+ * Numerics.  Products are exact and summed in fp32; a result is rounded once, when it is stored.  The low-rank
+ * intermediate A x stays in fp32.  NaN and infinities in one row or adapter reach only the rows that use it.
+ *
+ * Calls enqueue kernels on `stream` and return; they allocate nothing and may be captured into a graph.  `workspace` is device
+ * memory of at least vdb_projection_workspace_bytes, aligned to 16 bytes, its contents need not be kept; calls (and
+ * captured graphs) that may run at the same time need workspaces of their own. */
+typedef struct vdb_projection {
+    int64_t dim_in, dim_out;     /* 1 .. 65536 */
+    int32_t dtype;               /* VDB_F32, VDB_BF16, VDB_F16: type of rows, of incoming gradients and of every weight */
+    int32_t out_dtype;           /* type of what a call writes: dtype, or VDB_F32 */
+    int32_t groups;              /* matrices in w; adapted calls take one */
+    int32_t adapters;            /* adapters in a, b, scale; 0: none */
+    int32_t rank;                /* of every adapter, 1 .. 128 (smaller ones are filled up with zeros) */
+    int32_t reserved;            /* 0 */
+    const void*  w;              /* [groups][dim_out][dim_in] */
+    const void*  a;              /* [adapters][rank][dim_in] */
+    const void*  b;              /* [adapters][dim_out][rank] */
+    const float* scale;          /* [adapters], or NULL: 1 */
+} vdb_projection;
+
+/* Workspace of the calls below, for n rows in `segments` segments; a negative VDB_E* code if the arguments are refused. */
+int64_t vdb_projection_workspace_bytes(const vdb_projection* p, int64_t n, int64_t segments, int backward);
+/* y [n, dim_out] = x [n, dim_in] through the matrix of each row's group; offsets [groups + 1]. */
+int vdb_project_grouped_dev(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets,
+                            void* y, int64_t ldy, void* stream);
+/* dx [n, dim_in] = dy W[g], dw [groups][dim_out][dim_in] = sum of dy_i x_i^T over each group's rows (zero for a group
+ * without rows).  Either output may be NULL. */
+int vdb_project_grouped_backward_dev(const vdb_projection* p, int64_t n, const void* dy, int64_t lddy, const void* x,
+                                     int64_t ldx, const int64_t* offsets, void* dx, int64_t lddx, void* dw,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+/* adapter_ids [requests] int32 on the device: the adapter of each request; a request whose number is not in
+ * [0, adapters) goes through W alone.  Several requests may name one adapter. */
+int vdb_project_adapted_dev(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, int64_t requests,
+                            const int64_t* offsets, const int32_t* adapter_ids, void* y, int64_t ldy,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+/* dx = W^T dy + s A^T B^T dy, da [adapters][rank][dim_in] and db [adapters][dim_out][rank] summed over every row that
+ * used the adapter (zero for one that none used).  The shared matrix is taken as fixed; its gradient is that of
+ * vdb_project_grouped_backward_dev with one group.  dx may be NULL, and da and db together. */
+int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const void* dy, int64_t lddy, const void* x,
+                                     int64_t ldx, int64_t requests, const int64_t* offsets, const int32_t* adapter_ids,
+                                     void* dx, int64_t lddx, void* da, void* db,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+/* vdb_insert_dev of rows that go through the matrix of their group first (dim_out = the table's dimension; out_dtype is
+ * not looked at: the table receives the fp32 sums).  Every row has to have a group: offsets[0] = 0, offsets[groups] = n.
+ * Waits for its stream, like vdb_insert_dev. */
+int vdb_insert_projected_dev(const char* name, const vdb_projection* p, int64_t n, const void* x, int64_t ldx,
+                             const int64_t* offsets, const int64_t* ids_dev, void* stream);
+/* vdb_search_dev with queries that go through the shared matrix and their request's adapter first (out_dtype is not
+ * looked at: the search receives the fp32 sums).  Queries outside every request are searched as zero vectors. */
+int vdb_search_projected_dev(const char* name, const vdb_projection* p, int64_t nq, const void* x, int64_t ldx,
+                             int64_t requests, const int64_t* offsets, const int32_t* adapter_ids, int k,
+                             int64_t* out_ids_dev, float* out_scores_dev, int32_t* out_counts_dev, void* stream);
+
 /* ---- measurement hooks (bench.py) ------------------------------------------------------------ */
 /* on = 1: every launch of the dominant kernel (table scan, full batched pass) is bracketed by HIP
  * events on its stream; on = n > 1: every n-th launch (a pair of timing events costs about 10 us

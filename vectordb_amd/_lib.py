@@ -50,11 +50,34 @@ SIGNATURES = {
     "vdb_record_bytes": (C.c_int64, [C.c_int64, C.c_int]),
     "vdb_merge_records_dev": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p,
                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "vdb_projection_workspace_bytes": (C.c_int64, [C.c_void_p, C.c_int64, C.c_int64, C.c_int]),
+    "vdb_project_grouped_dev": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
+                                          C.c_void_p]),
+    "vdb_project_grouped_backward_dev": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                                   C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
+                                                   C.c_void_p]),
+    "vdb_project_adapted_dev": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+                                          C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "vdb_project_adapted_backward_dev": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                                   C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                                                   C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "vdb_insert_projected_dev": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                           C.c_void_p]),
+    "vdb_search_projected_dev": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
+                                           C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "vdb_bench_read_dev": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "vdb_prof_enable": (C.c_int, [C.c_int]),
     "vdb_prof_read": (C.c_int, [C.POINTER(C.c_double), _i64p]),
     "vdb_stats": (C.c_int, [_i64p, _i64p, _i64p]),
 }
+
+
+class ProjectionStruct(C.Structure):
+    """vdb_projection of include/vdb.h."""
+    _fields_ = [("dim_in", C.c_int64), ("dim_out", C.c_int64), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("groups", C.c_int32), ("adapters", C.c_int32), ("rank", C.c_int32), ("reserved", C.c_int32),
+                ("w", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p)]
+
 
 _lib = None
 

@@ -1,0 +1,65 @@
+// Parameters of the projection kernels (kernels_project.hip): learned maps of embeddings into a table's space.
+// Rows lie in segments: segment s holds rows [offsets[s], offsets[s + 1]).  Offsets come from device memory and are
+// clamped to [0, n] by every kernel, so that no value of them reaches memory outside the operands.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace vdb {
+
+constexpr int PROJ_MAX_RANK = 128;
+inline int proj_rank_pad(int rank) { return (rank + 15) / 16 * 16; }      // floats per row of a low-rank intermediate
+
+// y = x M^T with M [dim_y, dim_x] per segment or shared; the same kernel takes dx = dy M (M read down its columns).
+struct ProjRows {
+    const void* x; long long ldx;        // [n, K] rows, K contiguous
+    const void* w; long long w_group;    // matrix of segment 0; elements from one segment's matrix to the next (0: shared)
+    long long ldw;                       // elements between rows of the matrix as it is stored
+    bool w_by_k;                         // false: element (column, k) at column * ldw + k; true: at k * ldw + column
+    void* y; long long ldy;              // [n, N]
+    long long n; int N, K;
+    int dtype, out_dtype;
+    const long long* offsets; int segments;
+    // low-rank term: y_i += sum_q h[i][q] f[adapter][column][q]; null ids: none
+    const int* ids; int adapters;
+    const float* h; int rp;              // [n][rp], rp = proj_rank_pad(rank)
+    const void* f; long long f_adapter, f_col, f_rank;       // strides in elements
+    int rank;
+};
+
+// h[i][q] = scale[a] * sum_k x[i][k] f[a][q][k] for rows with an adapter; entries q in [rank, rp) are zero
+struct ProjShrink {
+    const void* x; long long ldx; long long n; int K;
+    const void* f; long long f_adapter, f_rank, f_k;
+    const float* scale;
+    float* h; int rp, rank;
+    int dtype;
+    const long long* offsets; int segments; const int* ids; int adapters;
+};
+
+// dw[g][m][c] = sum over the rows i of segment g of dy[i][m] x[i][c]
+struct ProjWeights {
+    const void* dy; long long lddy;
+    const void* x; long long ldx;
+    void* dw; int M, N;                  // [segments][M][N]
+    long long n; int dtype, out_dtype;
+    const long long* offsets; int segments;
+};
+
+// out[a][q][c] (or, by_col, out[a][c][q]) = sum over the rows i of adapter a of h[i][q] x[i][c]
+struct ProjFactor {
+    const float* h; int rp, rank;
+    const void* x; long long ldx; int N;
+    void* out; bool by_col;
+    long long n; int dtype, out_dtype;
+    const long long* offsets; int segments; const int* ids; int adapters;
+};
+
+hipError_t launch_proj_rows(const ProjRows& p, hipStream_t st);
+hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st);
+hipError_t launch_proj_weights(const ProjWeights& p, hipStream_t st);
+hipError_t launch_proj_factor(const ProjFactor& p, hipStream_t st);
+// rows [n, dim] of q outside every segment become zero
+hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st);
+
+}  // namespace vdb

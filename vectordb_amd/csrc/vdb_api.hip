@@ -2,7 +2,9 @@
 // See include/vdb.h for the contract of every entry point.
 #include "vdb_internal.h"
 #include "host_merge.h"
+#include "project.h"
 
+#include <algorithm>
 #include <atomic>
 #include <chrono>
 #include <cmath>
@@ -54,6 +56,7 @@ struct Workspace {
     DevBuf small;                                         // batched path: cnt | lost | thr0 | thr1
     DevBuf cand_h;                                        // scan path: list heads
     DevBuf q16;                                           // batched path, 16-bit tables: query hi | lo parts
+    DevBuf proj;                                          // projected queries behind their low-rank intermediate
     DevBuf qimg;                                          // batched path: tiled 16-bit image of the queries (ping-pong kernel)
     DevBuf q_raw, o_ids, o_scores, o_counts;              // staging of the host entry point (o_ids holds ids | scores | counts)
     void*  h_pin = nullptr;                               // pinned host mirror: queries | ids | scores | counts
@@ -964,7 +967,7 @@ int vdb_shutdown(void) {
     std::lock_guard<std::mutex> lk(G.mu);
     for (auto& w : G.free_ws) {
         for (DevBuf* b : {&w->qprep, &w->qinfo, &w->cand_s, &w->cand_t, &w->need_exact, &w->q_raw,
-                          &w->o_ids, &w->o_scores, &w->o_counts, &w->small, &w->cand_h, &w->q16, &w->qimg})
+                          &w->o_ids, &w->o_scores, &w->o_counts, &w->small, &w->cand_h, &w->q16, &w->qimg, &w->proj})
             if (b->p) (void)hipFree(b->p);
         if (w->h_pin) (void)hipHostFree(w->h_pin);
         if (w->stream) (void)hipStreamDestroy(w->stream);
@@ -2013,6 +2016,355 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
                               base + (size_t)nq * k * 12, stride,
                               (long long*)out_ids_dev, out_scores_dev, out_counts_dev, (hipStream_t)stream));
     return VDB_OK;
+}
+
+// ------------------------------------------------------------------------------ learned projections
+// Arguments are checked before the library's state, so that a refused call is refused the same way with and without a GPU.
+static int proj_check(const vdb_projection* p, int64_t n, int64_t segments, bool adapted) {
+    if (!p) return fail(VDB_EINVAL, "null projection");
+    if (p->dim_in < 1 || p->dim_in > 65536 || p->dim_out < 1 || p->dim_out > 65536)
+        return fail(VDB_EINVAL, "projection dimensions must be in [1, 65536]");
+    if (p->dtype != VDB_F32 && p->dtype != VDB_BF16 && p->dtype != VDB_F16) return fail(VDB_EINVAL, "unknown projection dtype");
+    if (p->out_dtype != p->dtype && p->out_dtype != VDB_F32) return fail(VDB_EINVAL, "out_dtype must be dtype or VDB_F32");
+    if (p->reserved != 0) return fail(VDB_EINVAL, "the reserved field of a projection must be 0");
+    if (p->groups < 1 || p->groups > 65536) return fail(VDB_EINVAL, "groups must be in [1, 65536]");
+    if (n < 0 || segments < 0) return fail(VDB_EINVAL, "negative number of rows or segments");
+    const uintptr_t e = p->dtype == VDB_F32 ? 4 : 2;
+    if (!p->w || (uintptr_t)p->w % e) return fail(VDB_EINVAL, "w is null or not aligned to its type");
+    if (adapted) {
+        if (p->groups != 1) return fail(VDB_EINVAL, "adapted calls take one shared matrix (groups = 1)");
+        if (p->adapters < 1 || p->adapters > 65535) return fail(VDB_EINVAL, "adapters must be in [1, 65535]");
+        if (p->rank < 1 || p->rank > PROJ_MAX_RANK) return fail(VDB_EINVAL, "rank must be in [1, 128]");
+        if (!p->a || !p->b || (uintptr_t)p->a % e || (uintptr_t)p->b % e) return fail(VDB_EINVAL, "a or b is null or not aligned to its type");
+        if ((uintptr_t)p->scale % 4) return fail(VDB_EINVAL, "scale is not aligned to its type");
+        if (segments > (1 << 24)) return fail(VDB_EINVAL, "more than 2^24 requests");
+    }
+    // every launch stays within 2^23 workgroups
+    const int64_t lim = (int64_t)1 << 23, td = 128;
+    const int64_t ct = (std::max(p->dim_in, p->dim_out) + td - 1) / td;
+    if (n > (lim - 8) / ct * 16 || (n / td + (adapted ? 1 : p->groups) + 1) * ct > lim - 8 ||
+        (int64_t)p->groups * ((p->dim_in + td - 1) / td) * ((p->dim_out + td - 1) / td) > lim)
+        return fail(VDB_EINVAL, "too many rows or groups for one call");
+    return VDB_OK;
+}
+
+// Rows [n, width] of `type`, ld apart.
+struct RowsArg {
+    const void* p;
+    int64_t ld, width;
+    int type;
+    const char* what;
+    int64_t esize() const { return type == VDB_F32 ? 4 : 2; }
+};
+
+static int rows_check(const RowsArg& r, int64_t n) {
+    if (!r.p) return fail(VDB_EINVAL, std::string("null ") + r.what);
+    if ((uintptr_t)r.p % r.esize()) return fail(VDB_EINVAL, std::string(r.what) + " is not aligned to its type");
+    if (r.ld < r.width || r.ld > ((int64_t)1 << 31)) return fail(VDB_EINVAL, std::string("leading dimension of ") + r.what + " is smaller than its rows or larger than 2^31");
+    (void)n;
+    return VDB_OK;
+}
+
+// Do rows a and b share an element?  Two views of one buffer with the same distance between rows may lie side by side.
+static bool rows_overlap(const RowsArg& a, const RowsArg& b, int64_t n) {
+    if (n < 1) return false;
+    const int64_t sa = a.ld * a.esize(), sb = b.ld * b.esize(), wa = a.width * a.esize(), wb = b.width * b.esize();
+    const uintptr_t a0 = (uintptr_t)a.p, a1 = a0 + (uintptr_t)((n - 1) * sa + wa);
+    const uintptr_t b0 = (uintptr_t)b.p, b1 = b0 + (uintptr_t)((n - 1) * sb + wb);
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (sa != sb) return true;
+    const int64_t d = (int64_t)((b0 > a0 ? b0 - a0 : a0 - b0) % (uintptr_t)sa);          // place of the later one in the earlier one's row
+    const int64_t we = b0 > a0 ? wa : wb, wl = b0 > a0 ? wb : wa;
+    return d < we || d + wl > sa;
+}
+
+static bool block_overlap(const void* p, int64_t bytes, const RowsArg& r, int64_t n) {
+    if (n < 1 || bytes < 1) return false;
+    const uintptr_t a0 = (uintptr_t)p, a1 = a0 + (uintptr_t)bytes;
+    const uintptr_t b0 = (uintptr_t)r.p, b1 = b0 + (uintptr_t)(((n - 1) * r.ld + r.width) * r.esize());
+    return a0 < b1 && b0 < a1;
+}
+
+static bool blocks_overlap(const void* p, int64_t pb, const void* q, int64_t qb) {
+    return p && q && pb > 0 && qb > 0 && (uintptr_t)p < (uintptr_t)q + (uintptr_t)qb && (uintptr_t)q < (uintptr_t)p + (uintptr_t)pb;
+}
+
+static int64_t proj_intermediate_bytes(const vdb_projection* p, int64_t n) {
+    return (int64_t)round_up((size_t)n * proj_rank_pad(p->rank) * sizeof(float), 256);
+}
+
+static int64_t proj_workspace(const vdb_projection* p, int64_t n, bool adapted, bool backward) {
+    return adapted ? proj_intermediate_bytes(p, n) * (backward ? 2 : 1) : 0;
+}
+
+static int workspace_check(void* ws, int64_t have, int64_t want) {
+    if (want == 0) return VDB_OK;
+    if (!ws || have < want) return fail(VDB_EINVAL, "workspace of " + std::to_string(have) + " bytes, " + std::to_string(want) + " needed");
+    if ((uintptr_t)ws % 16) return fail(VDB_EINVAL, "the workspace is not aligned to 16 bytes");
+    return VDB_OK;
+}
+
+static int segments_check(const int64_t* offsets, const int32_t* ids, int64_t segments, bool adapted) {
+    if (!offsets || (uintptr_t)offsets % 8) return fail(VDB_EINVAL, "offsets are null or not aligned to 8 bytes");
+    if (adapted && segments > 0 && (!ids || (uintptr_t)ids % 4)) return fail(VDB_EINVAL, "adapter ids are null or not aligned to 4 bytes");
+    return VDB_OK;
+}
+
+static ProjRows proj_forward(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets, int64_t segments,
+                             void* y, int64_t ldy, int out_dtype) {
+    ProjRows r{};
+    r.x = x; r.ldx = ldx; r.w = p->w; r.w_group = p->dim_out * p->dim_in; r.ldw = p->dim_in; r.w_by_k = false;
+    r.y = y; r.ldy = ldy; r.n = n; r.N = (int)p->dim_out; r.K = (int)p->dim_in; r.dtype = p->dtype; r.out_dtype = out_dtype;
+    r.offsets = (const long long*)offsets; r.segments = (int)segments;
+    return r;
+}
+
+// h = s x A^T, then y = x W^T + h B^T
+static hipError_t proj_adapted(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets, const int32_t* ids,
+                               int64_t requests, void* y, int64_t ldy, int out_dtype, float* h, hipStream_t st) {
+    ProjShrink s{};
+    s.x = x; s.ldx = ldx; s.n = n; s.K = (int)p->dim_in; s.dtype = p->dtype;
+    s.f = p->a; s.f_adapter = p->rank * p->dim_in; s.f_rank = p->dim_in; s.f_k = 1;
+    s.scale = p->scale; s.h = h; s.rank = p->rank; s.rp = proj_rank_pad(p->rank);
+    s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = ids; s.adapters = p->adapters;
+    hipError_t e = launch_proj_shrink(s, st);
+    if (e != hipSuccess) return e;
+    ProjRows r = proj_forward(p, n, x, ldx, offsets, requests, y, ldy, out_dtype);
+    r.w_group = 0; r.ids = ids; r.adapters = p->adapters; r.h = h; r.rp = s.rp; r.rank = p->rank;
+    r.f = p->b; r.f_adapter = p->dim_out * p->rank; r.f_col = p->rank; r.f_rank = 1;
+    return launch_proj_rows(r, st);
+}
+
+int64_t vdb_projection_workspace_bytes(const vdb_projection* p, int64_t n, int64_t segments, int backward) {
+    const bool adapted = p && p->adapters > 0;
+    const int rc = proj_check(p, n, segments, adapted);
+    if (rc) return rc;
+    return proj_workspace(p, n, adapted, backward != 0);
+}
+
+int vdb_project_grouped_dev(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets,
+                            void* y, int64_t ldy, void* stream) {
+    int rc = proj_check(p, n, 0, false);
+    if (rc) return rc;
+    if (n > 0) {
+        const RowsArg rx{x, ldx, p->dim_in, p->dtype, "x"}, ry{y, ldy, p->dim_out, p->out_dtype, "y"};
+        if ((rc = rows_check(rx, n)) || (rc = rows_check(ry, n)) || (rc = segments_check(offsets, nullptr, p->groups, false))) return rc;
+        if (rows_overlap(rx, ry, n) || block_overlap(p->w, (int64_t)p->groups * p->dim_in * p->dim_out * rx.esize(), ry, n) ||
+            block_overlap(offsets, (p->groups + 1) * (int64_t)8, ry, n))
+            return fail(VDB_EINVAL, "y shares memory with an input");
+    }
+    if ((rc = enter())) return rc;
+    if (n == 0) return VDB_OK;
+    VDB_HIP(launch_proj_rows(proj_forward(p, n, x, ldx, offsets, p->groups, y, ldy, p->out_dtype), (hipStream_t)stream));
+    return VDB_OK;
+}
+
+int vdb_project_grouped_backward_dev(const vdb_projection* p, int64_t n, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                     const int64_t* offsets, void* dx, int64_t lddx, void* dw, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+    int rc = proj_check(p, n, 0, false);
+    if (rc) return rc;
+    if (!dx && !dw) return fail(VDB_EINVAL, "both dx and dw are null");
+    const RowsArg rdy{dy, lddy, p->dim_out, p->dtype, "dy"}, rx{x, ldx, p->dim_in, p->dtype, "x"}, rdx{dx, lddx, p->dim_in, p->out_dtype, "dx"};
+    const int64_t wn = (int64_t)p->groups * p->dim_in * p->dim_out, dwb = wn * (p->out_dtype == VDB_F32 ? 4 : 2);
+    if (dw && (uintptr_t)dw % (p->out_dtype == VDB_F32 ? 4 : 2)) return fail(VDB_EINVAL, "dw is not aligned to its type");
+    if ((rc = segments_check(offsets, nullptr, p->groups, false))) return rc;
+    if (n > 0) {
+        if ((rc = rows_check(rdy, n)) || (dw && (rc = rows_check(rx, n))) || (dx && (rc = rows_check(rdx, n)))) return rc;
+        if (dx && (rows_overlap(rdx, rdy, n) || (dw && (rows_overlap(rdx, rx, n) || block_overlap(dw, dwb, rdx, n))) ||
+                   block_overlap(p->w, wn * rx.esize(), rdx, n) || block_overlap(offsets, (p->groups + 1) * (int64_t)8, rdx, n)))
+            return fail(VDB_EINVAL, "dx shares memory with an input or with dw");
+        if (dw && (block_overlap(dw, dwb, rdy, n) || block_overlap(dw, dwb, rx, n)))
+            return fail(VDB_EINVAL, "dw shares memory with an input");
+    }
+    if (dw && (blocks_overlap(dw, dwb, p->w, wn * rx.esize()) || blocks_overlap(dw, dwb, offsets, (p->groups + 1) * (int64_t)8)))
+        return fail(VDB_EINVAL, "dw shares memory with an input");
+    if ((rc = workspace_check(workspace, workspace_bytes, proj_workspace(p, n, false, true)))) return rc;
+    if ((rc = enter())) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (dx && n > 0) {
+        ProjRows r = proj_forward(p, n, dy, lddy, offsets, p->groups, dx, lddx, p->out_dtype);
+        r.w_by_k = true; r.N = (int)p->dim_in; r.K = (int)p->dim_out;
+        VDB_HIP(launch_proj_rows(r, st));
+    }
+    if (dw) {
+        ProjWeights w{};
+        w.dy = dy; w.lddy = lddy; w.x = x; w.ldx = ldx; w.dw = dw; w.M = (int)p->dim_out; w.N = (int)p->dim_in;
+        w.n = n; w.dtype = p->dtype; w.out_dtype = p->out_dtype; w.offsets = (const long long*)offsets; w.segments = p->groups;
+        VDB_HIP(launch_proj_weights(w, st));
+    }
+    return VDB_OK;
+}
+
+int vdb_project_adapted_dev(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, int64_t requests, const int64_t* offsets,
+                            const int32_t* adapter_ids, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
+    int rc = proj_check(p, n, requests, true);
+    if (rc) return rc;
+    const int64_t want = proj_workspace(p, n, true, false);
+    if (n > 0 && requests > 0) {
+        const RowsArg rx{x, ldx, p->dim_in, p->dtype, "x"}, ry{y, ldy, p->dim_out, p->out_dtype, "y"};
+        if ((rc = rows_check(rx, n)) || (rc = rows_check(ry, n)) || (rc = segments_check(offsets, adapter_ids, requests, true))) return rc;
+        const int64_t pair = (int64_t)p->adapters * p->rank * rx.esize();
+        if (rows_overlap(rx, ry, n) || block_overlap(p->w, p->dim_in * p->dim_out * rx.esize(), ry, n) ||
+            block_overlap(p->a, pair * p->dim_in, ry, n) || block_overlap(p->b, pair * p->dim_out, ry, n) ||
+            block_overlap(p->scale, p->scale ? p->adapters * (int64_t)4 : 0, ry, n) ||
+            block_overlap(offsets, (requests + 1) * 8, ry, n) || block_overlap(adapter_ids, requests * 4, ry, n))
+            return fail(VDB_EINVAL, "y shares memory with an input");
+        if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
+        if (block_overlap(workspace, want, rx, n) || block_overlap(workspace, want, ry, n))
+            return fail(VDB_EINVAL, "the workspace shares memory with x or y");
+    }
+    if ((rc = enter())) return rc;
+    if (n == 0 || requests == 0) return VDB_OK;
+    VDB_HIP(proj_adapted(p, n, x, ldx, offsets, adapter_ids, requests, y, ldy, p->out_dtype, (float*)workspace, (hipStream_t)stream));
+    return VDB_OK;
+}
+
+int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                     int64_t requests, const int64_t* offsets, const int32_t* adapter_ids, void* dx, int64_t lddx,
+                                     void* da, void* db, void* workspace, int64_t workspace_bytes, void* stream) {
+    int rc = proj_check(p, n, requests, true);
+    if (rc) return rc;
+    if (!da != !db) return fail(VDB_EINVAL, "da and db come together");
+    if (!dx && !da) return fail(VDB_EINVAL, "dx, da and db are all null");
+    const int64_t want = proj_workspace(p, n, true, true), half = proj_intermediate_bytes(p, n);
+    const RowsArg rdy{dy, lddy, p->dim_out, p->dtype, "dy"}, rx{x, ldx, p->dim_in, p->dtype, "x"}, rdx{dx, lddx, p->dim_in, p->out_dtype, "dx"};
+    const int64_t oe = p->out_dtype == VDB_F32 ? 4 : 2, pairs = (int64_t)p->adapters * p->rank, e = rx.esize();
+    const int64_t dab = pairs * p->dim_in * oe, dbb = pairs * p->dim_out * oe;
+    if (da && ((uintptr_t)da % oe || (uintptr_t)db % oe)) return fail(VDB_EINVAL, "da or db is not aligned to its type");
+    if ((rc = segments_check(offsets, adapter_ids, requests, true))) return rc;
+    const struct { const void* p; int64_t bytes; } in[] = {
+        {p->w, p->dim_in * p->dim_out * e}, {p->a, pairs * p->dim_in * e}, {p->b, pairs * p->dim_out * e},
+        {p->scale, p->scale ? p->adapters * (int64_t)4 : 0}, {offsets, (requests + 1) * 8}, {adapter_ids, requests * 4}};
+    if (n > 0) {
+        if ((rc = rows_check(rdy, n)) || (da && (rc = rows_check(rx, n))) || (dx && (rc = rows_check(rdx, n)))) return rc;
+        if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
+        bool bad = block_overlap(workspace, want, rdy, n) || (da && block_overlap(workspace, want, rx, n)) || (dx && block_overlap(workspace, want, rdx, n));
+        if (dx) {
+            bad = bad || rows_overlap(rdx, rdy, n) || (da && (rows_overlap(rdx, rx, n) || block_overlap(da, dab, rdx, n) || block_overlap(db, dbb, rdx, n)));
+            for (const auto& b : in) bad = bad || block_overlap(b.p, b.bytes, rdx, n);
+        }
+        if (da) bad = bad || block_overlap(da, dab, rdy, n) || block_overlap(da, dab, rx, n) || block_overlap(db, dbb, rdy, n) ||
+                      block_overlap(db, dbb, rx, n) || blocks_overlap(workspace, want, da, dab) || blocks_overlap(workspace, want, db, dbb);
+        if (bad) return fail(VDB_EINVAL, "an output or the workspace shares memory with another argument");
+    }
+    if (da) {
+        bool bad = blocks_overlap(da, dab, db, dbb);
+        for (const auto& b : in) bad = bad || blocks_overlap(b.p, b.bytes, da, dab) || blocks_overlap(b.p, b.bytes, db, dbb);
+        if (bad) return fail(VDB_EINVAL, "da or db shares memory with another argument");
+    }
+    if ((rc = enter())) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    float* const h = (float*)workspace;
+    float* const g = (float*)((char*)workspace + half);
+    const int rp = proj_rank_pad(p->rank);
+    ProjShrink s{};
+    s.n = n; s.dtype = p->dtype; s.scale = p->scale; s.rank = p->rank; s.rp = rp;
+    s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = adapter_ids; s.adapters = p->adapters;
+    // g = s dy B
+    s.x = dy; s.ldx = lddy; s.K = (int)p->dim_out; s.h = g;
+    s.f = p->b; s.f_adapter = p->dim_out * p->rank; s.f_rank = 1; s.f_k = p->rank;
+    VDB_HIP(launch_proj_shrink(s, st));
+    if (da) {
+        // h = s x A^T, again rather than kept from the forward pass
+        s.x = x; s.ldx = ldx; s.K = (int)p->dim_in; s.h = h;
+        s.f = p->a; s.f_adapter = p->rank * p->dim_in; s.f_rank = p->dim_in; s.f_k = 1;
+        VDB_HIP(launch_proj_shrink(s, st));
+    }
+    if (dx && n > 0) {
+        ProjRows r = proj_forward(p, n, dy, lddy, offsets, requests, dx, lddx, p->out_dtype);
+        r.w_group = 0; r.w_by_k = true; r.N = (int)p->dim_in; r.K = (int)p->dim_out;
+        r.ids = adapter_ids; r.adapters = p->adapters; r.h = g; r.rp = rp; r.rank = p->rank;
+        r.f = p->a; r.f_adapter = p->rank * p->dim_in; r.f_col = 1; r.f_rank = p->dim_in;
+        VDB_HIP(launch_proj_rows(r, st));
+    }
+    if (da) {
+        ProjFactor f{};
+        f.rp = rp; f.rank = p->rank; f.n = n; f.dtype = p->dtype; f.out_dtype = p->out_dtype;
+        f.offsets = (const long long*)offsets; f.segments = (int)requests; f.ids = adapter_ids; f.adapters = p->adapters;
+        f.h = g; f.x = x; f.ldx = ldx; f.N = (int)p->dim_in; f.out = da; f.by_col = false;
+        VDB_HIP(launch_proj_factor(f, st));
+        f.h = h; f.x = dy; f.ldx = lddy; f.N = (int)p->dim_out; f.out = db; f.by_col = true;
+        VDB_HIP(launch_proj_factor(f, st));
+    }
+    return VDB_OK;
+}
+
+int vdb_insert_projected_dev(const char* name, const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets,
+                             const int64_t* ids_dev, void* stream) {
+    int rc = proj_check(p, n, 0, false);
+    if (rc) return rc;
+    if (!name) return fail(VDB_EINVAL, "null table name");
+    if (n > 0) {
+        if ((rc = rows_check(RowsArg{x, ldx, p->dim_in, p->dtype, "x"}, n)) || (rc = segments_check(offsets, nullptr, p->groups, false))) return rc;
+        if (!ids_dev) return fail(VDB_EINVAL, "null ids");
+    }
+    if ((rc = enter())) return rc;
+    auto t = find_table(name);
+    if (!t) return fail(VDB_ENOTFOUND, std::string("no such table: ") + name);
+    if (p->dim_out != t->dim) return fail(VDB_EINVAL, "the projection's dim_out does not match the table's dimension");
+    if (n == 0) return VDB_OK;
+    hipStream_t st = (hipStream_t)stream;
+    try {
+        std::vector<int64_t> off((size_t)p->groups + 1);
+        VDB_HIP(hipMemcpyAsync(off.data(), offsets, off.size() * sizeof(int64_t), hipMemcpyDeviceToHost, st));
+        VDB_HIP(hipStreamSynchronize(st));
+        bool good = off.front() == 0 && off.back() == n;
+        for (size_t i = 1; i < off.size(); ++i) good = good && off[i - 1] <= off[i];
+        if (!good) return fail(VDB_EINVAL, "offsets must run from 0 to n without decreasing: every row of an insert needs a group");
+        // the projected rows wait in memory of the call's own: the insert publishes all of them at once
+        void* rows = nullptr;
+        if (hipMalloc(&rows, (size_t)n * t->dim * sizeof(float)) != hipSuccess) {
+            (void)hipGetLastError();
+            return fail(VDB_ENOMEM, "no memory for " + std::to_string(n) + " projected rows");
+        }
+        const hipError_t e = launch_proj_rows(proj_forward(p, n, x, ldx, offsets, p->groups, rows, t->dim, VDB_F32), st);
+        rc = e == hipSuccess ? insert_into(*t, n, (const float*)rows, (const long long*)ids_dev, false, false, 0, 0, st)
+                             : fail(VDB_EHIP, std::string("projection: ") + hipGetErrorString(e));
+        (void)hipStreamSynchronize(st);
+        (void)hipFree(rows);
+    } catch (const std::exception&) {
+        return fail(VDB_ENOMEM, "out of host memory");
+    }
+    return rc;
+}
+
+int vdb_search_projected_dev(const char* name, const vdb_projection* p, int64_t nq, const void* x, int64_t ldx, int64_t requests,
+                             const int64_t* offsets, const int32_t* adapter_ids, int k, int64_t* out_ids_dev, float* out_scores_dev,
+                             int32_t* out_counts_dev, void* stream) {
+    int rc = proj_check(p, nq, requests, true);
+    if (rc) return rc;
+    if ((rc = check_search_args(name, nq, x, k, out_ids_dev, out_scores_dev, out_counts_dev))) return rc;
+    if (nq > 0 && ((rc = rows_check(RowsArg{x, ldx, p->dim_in, p->dtype, "x"}, nq)) || (rc = segments_check(offsets, adapter_ids, requests, true))))
+        return rc;
+    if ((rc = enter())) return rc;
+    auto t = find_table(name);
+    if (!t) return fail(VDB_ENOTFOUND, std::string("no such table: ") + name);
+    if (p->dim_out != t->dim) return fail(VDB_EINVAL, "the projection's dim_out does not match the table's dimension");
+    if (nq == 0) return VDB_OK;
+    hipStream_t st = (hipStream_t)stream;
+    try {
+        std::unique_ptr<Workspace> ws;
+        if ((rc = acquire_ws(st, ws))) return rc;
+        const size_t hb = (size_t)proj_workspace(p, nq, true, false), qb = (size_t)nq * t->dim * sizeof(float);
+        rc = ensure(ws->proj, hb + qb, ws->last_stream);
+        if (rc == VDB_OK) {
+            float* const q = (float*)((char*)ws->proj.p + hb);
+            hipError_t e = launch_proj_zero_outside(q, t->dim, nq, (const long long*)offsets, (int)requests, st);
+            if (e == hipSuccess && requests > 0)
+                e = proj_adapted(p, nq, x, ldx, offsets, adapter_ids, requests, q, t->dim, VDB_F32, (float*)ws->proj.p, st);
+            if (e != hipSuccess) rc = fail(VDB_EHIP, std::string("projection: ") + hipGetErrorString(e));
+            else {
+                std::shared_lock<std::shared_mutex> tl(t->mu);
+                if (t->dropped) rc = fail(VDB_ENOTFOUND, "table was dropped");
+                else rc = search_core(*t, nq, q, k, (long long*)out_ids_dev, out_scores_dev, out_counts_dev, st, *ws);
+            }
+        }
+        release_ws(ws, st);
+    } catch (const std::exception&) {
+        return fail(VDB_ENOMEM, "out of host memory");
+    }
+    return rc;
 }
 
 int vdb_bench_read_dev(const void* buf_dev, int64_t bytes, int nt, int blocks, int threads, void* stream) {

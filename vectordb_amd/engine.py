@@ -201,6 +201,57 @@ class Engine:
                                              C.c_void_p(out_ids_ptr), C.c_void_p(out_scores_ptr),
                                              C.c_void_p(out_counts_ptr), C.c_void_p(stream)))
 
+    # ---- learned projections (vectordb_amd.projection.Projection; pointers are device addresses, ld* in elements)
+    def _proj(self, proj) -> int:
+        if proj.device != self.device:
+            raise VdbError(_lib.EINVAL, "the projection is on GPU %d, the engine on %d" % (proj.device, self.device))
+        return proj.ptr
+
+    def projection_workspace_bytes(self, proj, n: int, segments: int, backward: bool = False) -> int:
+        """Device memory that a call over n rows in `segments` sources or requests works in."""
+        size = self.lib.vdb_projection_workspace_bytes(self._proj(proj), n, segments, 1 if backward else 0)
+        if size < 0:
+            check(int(size))
+        return int(size)
+
+    def project_grouped_dev(self, proj, n: int, x_ptr: int, ldx: int, offsets_ptr: int, y_ptr: int, ldy: int,
+                            stream: int = 0) -> None:
+        """y[i] = w[g] x[i] for the rows of every group g: rows [offsets[g], offsets[g + 1])."""
+        check(self.lib.vdb_project_grouped_dev(self._proj(proj), n, x_ptr, ldx, offsets_ptr, y_ptr, ldy, stream))
+
+    def project_grouped_backward_dev(self, proj, n: int, dy_ptr: int, lddy: int, x_ptr: int, ldx: int, offsets_ptr: int,
+                                     dx_ptr: int, lddx: int, dw_ptr: int, ws_ptr: int = 0, ws_bytes: int = 0,
+                                     stream: int = 0) -> None:
+        """Gradients of project_grouped_dev; dx_ptr or dw_ptr may be 0."""
+        check(self.lib.vdb_project_grouped_backward_dev(self._proj(proj), n, dy_ptr, lddy, x_ptr, ldx, offsets_ptr,
+                                                        dx_ptr, lddx, dw_ptr, ws_ptr, ws_bytes, stream))
+
+    def project_adapted_dev(self, proj, n: int, x_ptr: int, ldx: int, requests: int, offsets_ptr: int, ids_ptr: int,
+                            y_ptr: int, ldy: int, ws_ptr: int, ws_bytes: int, stream: int = 0) -> None:
+        """y[i] = w x[i] + scale[a] b[a] (a[a] x[i]), a the adapter of the row's request (ids, int32; -1: none)."""
+        check(self.lib.vdb_project_adapted_dev(self._proj(proj), n, x_ptr, ldx, requests, offsets_ptr, ids_ptr, y_ptr, ldy,
+                                               ws_ptr, ws_bytes, stream))
+
+    def project_adapted_backward_dev(self, proj, n: int, dy_ptr: int, lddy: int, x_ptr: int, ldx: int, requests: int,
+                                     offsets_ptr: int, ids_ptr: int, dx_ptr: int, lddx: int, da_ptr: int, db_ptr: int,
+                                     ws_ptr: int, ws_bytes: int, stream: int = 0) -> None:
+        """Gradients of project_adapted_dev; dx_ptr may be 0, da_ptr and db_ptr may both be 0."""
+        check(self.lib.vdb_project_adapted_backward_dev(self._proj(proj), n, dy_ptr, lddy, x_ptr, ldx, requests,
+                                                        offsets_ptr, ids_ptr, dx_ptr, lddx, da_ptr, db_ptr, ws_ptr,
+                                                        ws_bytes, stream))
+
+    def insert_projected_dev(self, name: str, proj, n: int, x_ptr: int, ldx: int, offsets_ptr: int, ids_ptr: int,
+                             stream: int = 0) -> None:
+        """insert_dev of rows that go through the matrix of their group first."""
+        check(self.lib.vdb_insert_projected_dev(_name(name), self._proj(proj), n, x_ptr, ldx, offsets_ptr, ids_ptr, stream))
+
+    def search_projected_dev(self, name: str, proj, nq: int, x_ptr: int, ldx: int, requests: int, offsets_ptr: int,
+                             ids_ptr: int, k: int, out_ids_ptr: int, out_scores_ptr: int, out_counts_ptr: int,
+                             stream: int = 0) -> None:
+        """search_dev with queries that go through the shared matrix and their request's adapter first."""
+        check(self.lib.vdb_search_projected_dev(_name(name), self._proj(proj), nq, x_ptr, ldx, requests, offsets_ptr,
+                                                ids_ptr, k, out_ids_ptr, out_scores_ptr, out_counts_ptr, stream))
+
     def set_option(self, key: str, value: float) -> None:
         check(self.lib.vdb_set_option(_name(key), float(value)))
 
