@@ -239,6 +239,14 @@ def test_adapted_strides_and_alignment(engine, dtype, shift, pad):
         Case(140, 96, 160, [0, 50, 140], dtype, dtype, 3, 24, [1, 0], shift=shift, pad=pad).check(engine)
 
 
+@pytest.mark.parametrize("requests", [63, 64, 65, 128, 129, 256, 4096, 4097])
+def test_rows_behind_the_last_of_many_requests(engine, requests):
+    """The search for a row's request divides the offsets by 64 a step; rows in front of, between and behind all requests."""
+    n = requests + 40
+    ids = [i % 5 - 1 for i in range(requests)]
+    Case(n, 16, 24, list(range(7, 8 + requests)), "bf16", "f32", 4, 4, ids).check(engine)
+
+
 def test_large_values_of_the_low_rank_intermediate(engine):
     """A x beyond what fp16 holds, with B small enough that the product fits."""
     c = Case(33, 64, 48, [0, 20, 33], "f16", "f32", 2, 16, [1, 0], scale=False)

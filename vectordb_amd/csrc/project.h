@@ -4,11 +4,17 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include "../../include/vdb.h"
 
 namespace vdb {
 
 constexpr int PROJ_MAX_RANK = 128;
-inline int proj_rank_pad(int rank) { return (rank + 15) / 16 * 16; }      // floats per row of a low-rank intermediate
+// A low-rank intermediate h [n, rank], fp32, is handed to the kernel that multiplies it as parts of the rows' type that add up
+// to it: rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks for 16-bit types, 16 for fp32).
+__host__ __device__ constexpr int proj_parts(int dtype) { return dtype == VDB_F32 ? 1 : dtype == VDB_BF16 ? 3 : 2; }
+__host__ __device__ constexpr int proj_rank_pad(int rank, int dtype) {
+    return dtype == VDB_F32 ? (rank + 15) / 16 * 16 : (rank + 31) / 32 * 32;
+}
 
 // y = x M^T with M [dim_y, dim_x] per segment or shared; the same kernel takes dx = dy M (M read down its columns).
 struct ProjRows {
@@ -22,18 +28,20 @@ struct ProjRows {
     const long long* offsets; int segments;
     // low-rank term: y_i += sum_q h[i][q] f[adapter][column][q]; null ids: none
     const int* ids; int adapters;
-    const float* h; int rp;              // [n][rp], rp = proj_rank_pad(rank)
+    const void* h;                       // [n][proj_parts][proj_rank_pad]
+    const float* h_scale;                // fp16: [n], what the parts of a row have to be multiplied with
     const void* f; long long f_adapter, f_col, f_rank;       // strides in elements
     int rank;
 };
 
-// h[i][q] = scale[a] * sum_k x[i][k] f[a][q][k] for rows with an adapter; entries q in [rank, rp) are zero
+// h[i][q] = scale[a] * sum_k x[i][k] f[a][q][k] for rows with an adapter; padding is zero
 struct ProjShrink {
     const void* x; long long ldx; long long n; int K;
     const void* f; long long f_adapter, f_rank, f_k;
     const float* scale;
-    float* h; int rp, rank;
-    int dtype;
+    void* h; float* h_scale;             // parts, see ProjRows; null: not wanted
+    float* h32; int rp32;                // [n][rp32] fp32; null: not wanted
+    int rank, dtype;
     const long long* offsets; int segments; const int* ids; int adapters;
 };
 
@@ -56,6 +64,12 @@ struct ProjFactor {
 };
 
 hipError_t launch_proj_rows(const ProjRows& p, hipStream_t st);
+hipError_t launch_proj_rows_f32(const ProjRows& p, hipStream_t st);
+hipError_t launch_proj_rows_bf16(const ProjRows& p, hipStream_t st);
+hipError_t launch_proj_rows_f16(const ProjRows& p, hipStream_t st);
+hipError_t launch_proj_weights_f32(const ProjWeights& p, hipStream_t st);
+hipError_t launch_proj_weights_bf16(const ProjWeights& p, hipStream_t st);
+hipError_t launch_proj_weights_f16(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st);
 hipError_t launch_proj_weights(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_factor(const ProjFactor& p, hipStream_t st);

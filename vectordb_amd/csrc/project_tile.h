@@ -1,0 +1,557 @@
+// Device side of the learned projections: segments, operand tiles in LDS, the tiled products and the low-rank term.
+// Included by one source file for each type (kernels_project_*.hip) and by kernels_project.hip.
+#pragma once
+#include "vdb_internal.h"
+#include "project.h"
+
+namespace vdb {
+
+typedef float pj_f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pj_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pj_f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int pj_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short pj_u16x8 __attribute__((ext_vector_type(8)));
+typedef short pj_s16x4 __attribute__((ext_vector_type(4)));
+
+#define PJ_GLOBAL __attribute__((address_space(1)))
+#define PJ_LOCAL __attribute__((address_space(3)))
+
+// Sixteen zero bytes: the source of every 16-byte piece of a tile that lies outside its operand.
+static __device__ __align__(16) const unsigned int pj_zero16[4] = {0, 0, 0, 0};
+
+template <int DT> struct PJ {            // 16-bit types
+    static constexpr int E = 2;
+    typedef unsigned short T;
+};
+template <> struct PJ<VDB_F32> {
+    static constexpr int E = 4;
+    typedef float T;
+};
+
+template <int DT> __device__ __forceinline__ float pj_to_f32(typename PJ<DT>::T v) {
+    if constexpr (DT == VDB_F32) return v;
+    else if constexpr (DT == VDB_BF16) return __uint_as_float((unsigned)v << 16);
+    else return (float)__builtin_bit_cast(_Float16, v);
+}
+// rounded once, to nearest even
+template <int DT> __device__ __forceinline__ typename PJ<DT>::T pj_from_f32(float v) {
+    if constexpr (DT == VDB_F32) return v;
+    else if constexpr (DT == VDB_BF16) return __builtin_bit_cast(unsigned short, (__bf16)v);
+    else return __builtin_bit_cast(unsigned short, (_Float16)v);
+}
+
+// ------------------------------------------------------------------------------------------- segments
+__device__ __forceinline__ long long pj_clamp(long long v, long long n) { return v < 0 ? 0 : v > n ? n : v; }
+
+// Which tile of TM rows workgroup `bid` of a grouped product works on: tiles are numbered segment by segment
+// (ceil(size / TM) each), column tiles run fastest, and the numbers are dealt to the eight XCDs in contiguous runs
+// (workgroup b runs on XCD b % 8), so that the column tiles that share rows share an L2.
+// Every wave does this by itself, 64 segments at a time.  Returns false for workgroups past the last tile.
+__device__ __forceinline__ bool pj_find_tile(const long long* offsets, int segments, long long n, int tm, int col_tiles,
+                                             unsigned bid, int& seg, long long& row0, long long& row1, int& col) {
+    const int lane = threadIdx.x & 63;
+    long long total = 0;
+    for (int s0 = 0; s0 < segments; s0 += 64) {
+        const int s = s0 + lane;
+        long long t = 0;
+        if (s < segments) {
+            const long long b = pj_clamp(offsets[s], n), e = pj_clamp(offsets[s + 1], n);
+            t = e > b ? (e - b + tm - 1) / tm : 0;
+        }
+        for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o);
+        total += t;
+    }
+    const long long all = total * col_tiles, run = (all + 7) / 8;
+    const long long idx = (long long)(bid >> 3);
+    if (idx >= run) return false;
+    const long long id = (long long)(bid & 7) * run + idx;
+    if (id >= all) return false;
+    col = (int)(id % col_tiles);
+    const long long want = id / col_tiles;
+    long long before = 0;
+    for (int s0 = 0; s0 < segments; s0 += 64) {
+        const int s = s0 + lane;
+        long long b = 0, e = 0, t = 0;
+        if (s < segments) {
+            b = pj_clamp(offsets[s], n); e = pj_clamp(offsets[s + 1], n);
+            t = e > b ? (e - b + tm - 1) / tm : 0;
+        }
+        long long inc = t;
+        for (int o = 1; o < 64; o <<= 1) { const long long u = __shfl_up(inc, o); if (lane >= o) inc += u; }
+        const bool mine = before + inc - t <= want && want < before + inc;
+        const unsigned long long m = __ballot(mine);
+        if (m) {
+            const int src = __builtin_ctzll(m);
+            seg = s0 + src;
+            row0 = __shfl(b + (want - (before + inc - t)) * tm, src);
+            row1 = __shfl(e, src);
+            return true;
+        }
+        before += __shfl(inc, 63);
+    }
+    return false;
+}
+
+// First segment whose end lies behind `row` (offsets do not decrease); `segments` if there is none.  Called by whole
+// waves: 64 ends are compared at a time, so that a search costs one load for each factor of 64.
+__device__ __forceinline__ int pj_first_segment(const long long* offsets, int segments, long long row) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = segments;                       // the answer lies in [lo, hi]
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64;
+        const int at = lo + (lane + 1) * step - 1;   // last segment of this lane's share
+        const bool behind = at >= hi || offsets[at + 1] > row;
+        const unsigned long long m = __ballot(behind);
+        const int k = m ? __builtin_ctzll(m) : 64;   // none: the 64 shares end at hi, and every segment lies before the row
+        const int nlo = lo + k * step, nhi = lo + (k + 1) * step - 1;
+        lo = nlo < hi ? nlo : hi;
+        hi = nhi < hi ? nhi : hi;
+    }
+    return lo;
+}
+
+// Requests with an adapter that meet rows [r0, r1): visited one by one by the whole wave, 64 loaded at a time.
+template <typename F>
+__device__ __forceinline__ void pj_each_request(const long long* offsets, const int* ids, int segments, int adapters, long long n,
+                                                long long r0, long long r1, F&& visit) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = pj_first_segment(offsets, segments, r0); s0 < segments; s0 += 64) {
+        const int s = s0 + lane;
+        long long b = n, e = 0;
+        int a = -1;
+        if (s < segments) { b = pj_clamp(offsets[s], n); e = pj_clamp(offsets[s + 1], n); a = ids[s]; }
+        unsigned long long m = __ballot(e > b && b < r1 && e > r0 && a >= 0 && a < adapters);
+        const bool last = __ballot(s < segments && b >= r1) != 0;
+        while (m) {
+            const int src = __builtin_ctzll(m);
+            m &= m - 1;
+            visit(__shfl(b, src), __shfl(e, src), __builtin_amdgcn_readlane(a, src));
+        }
+        if (last) break;
+    }
+}
+
+// ------------------------------------------------------------------------------------------- tiles in LDS
+// One operand tile: R = 64 or 128 rows (or columns) of the product by 128 bytes of the contracted axis, kept as it lies in
+// memory in 16-byte pieces whose place is swizzled so that the fragment reads below touch every bank once:
+//   contiguous along k (BYK = false): row r is 128 bytes, piece c sits in slot c ^ ((r >> 1) & 7)
+//   contiguous along the rows (BYK = true): one line per k, piece c of line k in slot c ^ pj_line_swizzle(k)
+constexpr int PJ_THREADS = 256;
+constexpr int pj_tile_bytes(int R) { return R * 128; }
+
+template <int DT, int R> __device__ __forceinline__ int pj_line_swizzle(int k) {
+    if constexpr (DT == VDB_F32) return (k >> 2 & 3) << 2;                       // 64-byte spans: the four lane groups read lines k, k + 4, ...
+    else if constexpr (R == 128) return ((k & 3) | (k >> 3 & 1) << 2) << 1;      // 32-byte spans of a 256-byte line
+    else return ((k >> 1 & 1) | (k >> 3 & 1) << 1) << 1;                         // 32-byte spans of a 128-byte line, two lines cover the banks
+}
+
+template <int DT, bool BYK, int R> struct PJOperand {
+    typedef typename PJ<DT>::T T;
+    static constexpr int E = PJ<DT>::E, V = 16 / E, KT = 128 / E, P = R / 32;    // P: pieces per thread
+    static constexpr int PL = R * E / 16;                                        // BYK: pieces per line
+    const T* src[P];
+    long long step[P];
+    int kpos[P];                 // k of the piece within a tile
+    int rem[P];                  // elements of the piece that lie in the operand's rows (V or 0 if !BYK)
+
+    // rows r0 .. r0 + R - 1 of [0, rows), k from 0
+    __device__ __forceinline__ void init(const T* base, long long ld, long long r0, long long rows) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int p = i * PJ_THREADS + (int)threadIdx.x;
+            if constexpr (!BYK) {
+                const int r = p >> 3, c = (p & 7) ^ ((r >> 1) & 7);
+                kpos[i] = c * V;
+                rem[i] = r0 + r < rows ? V : 0;
+                src[i] = base + (rem[i] ? (r0 + r) * ld + c * V : 0);
+                step[i] = rem[i] ? KT : 0;
+            } else {
+                const int k = p / PL, c = p % PL ^ pj_line_swizzle<DT, R>(k);
+                kpos[i] = k;
+                const long long left = rows - (r0 + c * V);
+                rem[i] = left >= V ? V : left > 0 ? (int)left : 0;
+                src[i] = base + (rem[i] ? (long long)k * ld + r0 + c * V : 0);
+                step[i] = rem[i] ? KT * ld : 0;
+            }
+        }
+    }
+    // the next KT elements of the contracted axis, of which `kleft` lie in the operand: one load per piece whatever kleft is
+    template <bool VEC> __device__ __forceinline__ void stage(char* lds, int kleft) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            char* const wave_dst = lds + (i * PJ_THREADS + ((int)threadIdx.x & ~63)) * 16;
+            if constexpr (VEC) {
+                const T* s = rem[i] && kpos[i] < kleft ? src[i] : (const T*)pj_zero16;
+                __builtin_amdgcn_global_load_lds((const PJ_GLOBAL void*)s, (PJ_LOCAL void*)wave_dst, 16, 0, 0);
+            } else {
+                T v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const bool ok = BYK ? (j < rem[i] && kpos[i] < kleft) : (rem[i] && kpos[i] + j < kleft);
+                    v[j] = ok ? src[i][j] : (T)0;
+                }
+                T* d = (T*)(wave_dst + ((int)threadIdx.x & 63) * 16);
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[j] = v[j];
+            }
+            src[i] += step[i];
+        }
+    }
+};
+
+// Fragments of B times 16 rows from `row` (a multiple of 16): lane l holds row + l % 16 and, of the step's 64 bytes of k, the 16
+// bytes number l / 16 (16-bit: k = 8 (l / 16) + 0..7; fp32: k = 4 (l / 16) + 0..3, one element for each of four products).
+template <int DT, bool BYK, int R, int B>
+__device__ __forceinline__ void pj_fragments(const char* lds, int row, int kk, pj_u32x4 (&f)[B]) {
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    constexpr int LINE = R * PJ<DT>::E;
+    if constexpr (!BYK) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int r = row + i * 16 + li;
+            f[i] = *(const pj_u32x4*)(lds + r * 128 + (((kk * 4 + lh) ^ ((r >> 1) & 7)) << 4));
+        }
+    } else if constexpr (DT == VDB_F32) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int c = ((row + i * 16 + li) >> 2) ^ (lh << 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                f[i][j] = *(const unsigned*)(lds + (kk * 16 + lh * 4 + j) * LINE + (c << 4) + (li & 3) * 4);
+        }
+    } else {
+        // ds_read_b64_tr_b16: sixteen lanes read a block of 4 k x 16 rows, lane i the 8 bytes number i % 4 of line i / 4, and get
+        // column i of the block; lines k and k + 4 have the same swizzle.  The reads and their wait are one asm block: through
+        // the builtin the compiler waits for every load into LDS in flight first.
+        const int k = lh * 8 + (li >> 2), swz = pj_line_swizzle<DT, R>(k);
+        const unsigned line = (unsigned)(uintptr_t)(PJ_LOCAL const char*)lds + (unsigned)((kk * 32 + k) * LINE + (li & 1) * 8);
+        unsigned at[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) at[i] = line + (unsigned)(((((row + i * 16) >> 3) + ((li & 3) >> 1)) ^ swz) << 4);
+        unsigned long long v[B][2];
+        if constexpr (B == 4)
+            asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+                         "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]), "=&v"(v[3][1])
+                         : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(4 * LINE) : "memory");
+        else
+            asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                         "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+                         "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+                         : "v"(at[0]), "v"(at[1]), "n"(4 * LINE) : "memory");
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            struct two { unsigned long long a, b; } t = {v[i][0], v[i][1]};
+            f[i] = __builtin_bit_cast(pj_u32x4, t);
+        }
+    }
+}
+
+// D[n][m] += sum_k a[n][k] b[m][k] over the step's 64 bytes of k; lane l of D holds m = l % 16, n = 4 (l / 16) + 0..3
+template <int DT> __device__ __forceinline__ pj_f32x4 pj_mfma(const pj_u32x4& a, const pj_u32x4& b, pj_f32x4 c) {
+    if constexpr (DT == VDB_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pj_bf16x8, a), __builtin_bit_cast(pj_bf16x8, b), c, 0, 0, 0);
+    else if constexpr (DT == VDB_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pj_f16x8, a), __builtin_bit_cast(pj_f16x8, b), c, 0, 0, 0);
+    else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    }
+}
+
+// Stores the four consecutive columns that a lane holds of one row; `left` of them lie in the output.
+template <int DT> __device__ __forceinline__ void pj_store4(void* out, long long at, const pj_f32x4& v, long long left, bool vec) {
+    typedef typename PJ<DT>::T T;
+    T* p = (T*)out + at;
+    T t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = pj_from_f32<DT>(v[j]);
+    if (vec && left >= 4) {
+        if constexpr (DT == VDB_F32) *(pj_f32x4*)p = v;
+        else { pj_s16x4 s = {(short)t[0], (short)t[1], (short)t[2], (short)t[3]}; *(pj_s16x4*)p = s; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (j < left) p[j] = t[j];
+    }
+}
+
+// ------------------------------------------------------------------------------------------- tiled products
+// Waits until at most N of this wave's loads are in flight and all its LDS reads have returned, then meets the other waves.
+template <int N> __device__ __forceinline__ void pj_wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Tiles of a launch: 64 x 64 with four stages of k in flight where there are few of them, 128 x 128 with two stages and
+// two workgroups on a CU where there are many (see pj_small_tiles).
+template <int R> struct PJRing {
+    static constexpr int STAGES = R == 64 ? 4 : 2;
+    static constexpr int BYTES = STAGES * 2 * pj_tile_bytes(R);
+};
+
+// One R x R output tile: a ring of LDS stages, each the next 128 bytes of k of both operands.  The loads of a stage are
+// issued STAGES - 1 steps ahead; every step issues the same number of them (zeros past the end), so that the wait can count.
+template <int DT, bool MK, bool NK, bool VEC, int R>
+struct PJProduct {
+    static constexpr int KT = 128 / PJ<DT>::E, B = R / 32, S = PJRing<R>::STAGES, TB = pj_tile_bytes(R);
+    PJOperand<DT, MK, R> om;
+    PJOperand<DT, NK, R> on;
+    long long left;              // of k, not yet staged
+    int tiles;
+
+    __device__ __forceinline__ void next(char* lds, int stage) {
+        const int l = left < KT ? (left > 0 ? (int)left : 0) : KT;
+        om.template stage<VEC>(lds + stage * 2 * TB, l);
+        on.template stage<VEC>(lds + stage * 2 * TB + TB, l);
+        left -= KT;
+    }
+    __device__ __forceinline__ void begin(long long K, char* lds) {
+        left = K;
+        tiles = (int)((K + KT - 1) / KT);
+        if (tiles > 0)
+#pragma unroll
+            for (int i = 0; i < S - 1; ++i) next(lds, i);
+    }
+    // acc += om on^T; the wave's block is rows wm * R/2.., columns wn * R/2..
+    __device__ __forceinline__ void run(char* lds, int wm, int wn, pj_f32x4 (&acc)[B][B]) {
+        constexpr int L = 2 * PJOperand<DT, MK, R>::P;          // loads per stage and thread
+        int cur = 0;
+        for (int t = 0; t < tiles; ++t) {
+            pj_wait_and_meet<VEC ? (S - 2) * L : 0>();
+            next(lds, cur == 0 ? S - 1 : cur - 1);
+            const char* lm = lds + cur * 2 * TB;
+            const char* ln = lm + TB;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                pj_u32x4 fm[B], fn[B];
+                pj_fragments<DT, MK, R, B>(lm, wm * (R / 2), kk, fm);
+                pj_fragments<DT, NK, R, B>(ln, wn * (R / 2), kk, fn);
+#pragma unroll
+                for (int i = 0; i < B; ++i)
+#pragma unroll
+                    for (int j = 0; j < B; ++j) acc[i][j] = pj_mfma<DT>(fn[j], fm[i], acc[i][j]);
+            }
+            cur = cur + 1 == S ? 0 : cur + 1;
+        }
+        // nothing may still be on its way into LDS when the workgroup's memory goes to another one
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+};
+
+// Low-rank term of a wave's block, before the main product: for every request that meets 16 of its rows, h f^T, taken over
+// by the rows of that request only, so that what one adapter holds never reaches another request's rows.  The fp32
+// intermediate h comes in parts of the rows' type that add up to it (bf16: three; fp16: two, with a power of two for each row
+// that brings its largest entry to 1/2..1, as fp16 could not hold it; see pj_store_parts), so that the term runs on
+// the 16-bit matrix unit without rounding h.
+template <int DT, bool FV, int B>
+__device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, int colb, pj_f32x4 (&acc)[B][B]) {
+    typedef typename PJ<DT>::T T;
+    constexpr int V = 16 / PJ<DT>::E, QS = 4 * V, NP = proj_parts(DT);
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    const int rp = proj_rank_pad(p.rank, DT);
+    pj_each_request(p.offsets, p.ids, p.segments, p.adapters, p.n, row, row + B * 16, [&](long long b, long long e, int a) {
+        const T* f = (const T*)p.f + (long long)a * p.f_adapter;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const long long r0 = row + i * 16, m = r0 + li;
+            if (b >= r0 + 16 || e <= r0) continue;
+            const T* h = (const T*)p.h + (m < p.n ? m : p.n - 1) * (NP * rp);
+            pj_f32x4 t[B] = {};
+            for (int q = 0; q < p.rank; q += QS) {
+                pj_u32x4 hv[NP];
+#pragma unroll
+                for (int u = 0; u < NP; ++u) hv[u] = *(const pj_u32x4*)(h + u * rp + q + lh * V);
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    const int col = colb + j * 16 + li, r = q + lh * V;
+                    const T* fc = f + (long long)(col < p.N ? col : p.N - 1) * p.f_col;
+                    union { T t[V]; pj_u32x4 v; } fv;
+                    if constexpr (FV) fv.v = *(const pj_u32x4*)(r < p.rank ? fc + r : (const T*)pj_zero16);
+                    else
+#pragma unroll
+                        for (int u = 0; u < V; ++u) fv.t[u] = r + u < p.rank ? fc[(long long)(r + u) * p.f_rank] : (T)0;
+#pragma unroll
+                    for (int u = NP - 1; u >= 0; --u) t[j] = pj_mfma<DT>(fv.v, hv[u], t[j]);
+                }
+            }
+            if (m >= b && m < e) {
+                const float sc = DT == VDB_F16 ? p.h_scale[m] : 1.f;
+#pragma unroll
+                for (int j = 0; j < B; ++j) acc[i][j] = DT == VDB_F16 ? t[j] * sc : t[j];
+            }
+        }
+    });
+}
+
+struct PJRowsArgs {
+    ProjRows p;
+    int col_tiles;
+    bool vec_out;
+};
+
+template <int DT, int ODT, bool NK, bool VEC, bool ADAPT, bool FV, int R>
+__global__ void __launch_bounds__(PJ_THREADS, 2)
+proj_rows_kernel(PJRowsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char pj_lds[];
+    typedef typename PJ<DT>::T T;
+    constexpr int B = R / 32;
+    const ProjRows& p = a.p;
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+    long long row0, row1, first = 0;         // rows of this tile: [max(row0, first), row1)
+    int seg = 0, col;
+    if constexpr (ADAPT) {
+        // one matrix for all rows: tiles over the rows from the first segment's start to the last one's end
+        const long long begin = pj_clamp(p.offsets[0], p.n), end = pj_clamp(p.offsets[p.segments], p.n);
+        if (end <= begin) return;
+        const long long t0 = begin / R, tiles = (end + R - 1) / R - t0;
+        const long long all = tiles * a.col_tiles, run = (all + 7) / 8, idx = blockIdx.x >> 3;
+        const long long id = (long long)(blockIdx.x & 7) * run + idx;
+        if (idx >= run || id >= all) return;
+        col = (int)(id % a.col_tiles);
+        row0 = (t0 + id / a.col_tiles) * R;
+        first = begin; row1 = end;
+    } else {
+        if (!pj_find_tile(p.offsets, p.segments, p.n, R, a.col_tiles, blockIdx.x, seg, row0, row1, col)) return;
+    }
+    const int col0 = col * R;
+    pj_f32x4 acc[B][B] = {};
+    PJProduct<DT, false, NK, VEC, R> prod;
+    prod.om.init((const T*)p.x, p.ldx, row0, row1);
+    prod.on.init((const T*)p.w + (long long)seg * p.w_group, p.ldw, col0, p.N);
+    prod.begin(p.K, pj_lds);
+    if constexpr (ADAPT) pj_low_rank<DT, FV, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), acc);
+    prod.run(pj_lds, wm, wn, acc);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const long long m = row0 + wm * (R / 2) + i * 16 + li;
+        if (m >= row1 || m < first) continue;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const int c = col0 + wn * (R / 2) + j * 16 + lh * 4;
+            if (c < p.N) pj_store4<ODT>(p.y, m * p.ldy + c, acc[i][j], p.N - c, a.vec_out);
+        }
+    }
+}
+
+struct PJWeightsArgs {
+    ProjWeights p;
+    int m_tiles, n_tiles;
+    bool vec_out;
+};
+
+template <int DT, int ODT, bool VEC, int R>
+__global__ void __launch_bounds__(PJ_THREADS, 2)
+proj_weights_kernel(PJWeightsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char pj_lds[];
+    typedef typename PJ<DT>::T T;
+    constexpr int B = R / 32;
+    const ProjWeights& p = a.p;
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+    const int seg = blockIdx.x / (a.m_tiles * a.n_tiles), rest = blockIdx.x % (a.m_tiles * a.n_tiles);
+    const int m0 = rest / a.n_tiles * R, n0 = rest % a.n_tiles * R;
+    const long long b = pj_clamp(p.offsets[seg], p.n), e = pj_clamp(p.offsets[seg + 1], p.n);
+    pj_f32x4 acc[B][B] = {};
+    PJProduct<DT, true, true, VEC, R> prod;
+    prod.om.init((const T*)p.dy + b * p.lddy, p.lddy, m0, p.M);
+    prod.on.init((const T*)p.x + b * p.ldx, p.ldx, n0, p.N);
+    prod.begin(e > b ? e - b : 0, pj_lds);
+    prod.run(pj_lds, wm, wn, acc);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const int m = m0 + wm * (R / 2) + i * 16 + li;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const int c = n0 + wn * (R / 2) + j * 16 + lh * 4;
+            if (c < p.N) pj_store4<ODT>(p.dw, ((long long)seg * p.M + m) * p.N + c, acc[i][j], p.N - c, a.vec_out);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- launches of one type
+static inline bool pj_aligned(const void* ptr, long long ld, int esize, int bytes) {
+    return (uintptr_t)ptr % bytes == 0 && ld * esize % bytes == 0;
+}
+
+template <typename K, typename A>
+static hipError_t pj_launch(K kernel, dim3 grid, size_t lds, const A& args, hipStream_t st) {
+    hipLaunchKernelGGL(kernel, grid, dim3(PJ_THREADS), lds, st, args);
+    return hipGetLastError();
+}
+
+// 64 x 64 tiles where 128 x 128 ones would leave CUs without work.
+static inline bool pj_small_tiles(long long tiles128) { return tiles128 < 256; }
+
+template <int DT, int ODT, int R>
+static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
+    PJRowsArgs a;
+    a.p = p;
+    a.col_tiles = (p.N + R - 1) / R;
+    constexpr int E = PJ<DT>::E, V = 16 / E;
+    a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 4 * PJ<ODT>::E);
+    const long long row_tiles = p.ids ? (p.n + R - 1) / R : p.n / R + p.segments;
+    const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
+    const size_t lds = PJRing<R>::BYTES;
+    // low-rank factor: forward its ranks are contiguous, backward its columns
+    const bool fv = p.ids && p.f_rank == 1 && p.rank % V == 0 && (uintptr_t)p.f % 16 == 0;
+#define PJ_ROWS(NK, VEC)                                                                              \
+    (!p.ids ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, false, R>, grid, lds, a, st)        \
+     : fv   ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, !NK, R>, grid, lds, a, st)           \
+            : pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, false, R>, grid, lds, a, st))
+    if constexpr (R == 128) return p.w_by_k ? PJ_ROWS(true, true) : PJ_ROWS(false, true);
+    else {
+        if (p.w_by_k) return vec ? PJ_ROWS(true, true) : PJ_ROWS(true, false);
+        return vec ? PJ_ROWS(false, true) : PJ_ROWS(false, false);
+    }
+#undef PJ_ROWS
+}
+
+template <int DT, int ODT>
+static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
+    constexpr int E = PJ<DT>::E, V = 16 / E;
+    const bool vec = pj_aligned(p.x, p.ldx, E, 16) && pj_aligned(p.w, p.ldw, E, 16) && p.w_group % V == 0 &&
+                     p.K % V == 0 && (!p.w_by_k || p.N % V == 0);
+    const long long tiles = ((p.n + 127) / 128 + (p.ids ? 0 : p.segments / 2)) * ((p.N + 127) / 128);
+    return vec && !pj_small_tiles(tiles) ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
+}
+
+template <int DT, int ODT, int R>
+static hipError_t pj_weights_sized(const ProjWeights& p, bool vec, hipStream_t st) {
+    PJWeightsArgs a;
+    a.p = p;
+    a.m_tiles = (p.M + R - 1) / R;
+    a.n_tiles = (p.N + R - 1) / R;
+    a.vec_out = pj_aligned(p.dw, p.N, PJ<ODT>::E, 4 * PJ<ODT>::E);
+    const dim3 grid((unsigned)((long long)p.segments * a.m_tiles * a.n_tiles));
+    if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, R>, grid, PJRing<R>::BYTES, a, st);
+    else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, R>, grid, PJRing<R>::BYTES, a, st)
+                    : pj_launch(proj_weights_kernel<DT, ODT, false, R>, grid, PJRing<R>::BYTES, a, st);
+}
+
+template <int DT, int ODT>
+static hipError_t pj_weights(const ProjWeights& p, hipStream_t st) {
+    constexpr int E = PJ<DT>::E, V = 16 / E;
+    const bool vec = pj_aligned(p.dy, p.lddy, E, 16) && pj_aligned(p.x, p.ldx, E, 16) && p.M % V == 0 && p.N % V == 0;
+    const long long tiles = (long long)p.segments * ((p.M + 127) / 128) * ((p.N + 127) / 128);
+    return vec && !pj_small_tiles(tiles) ? pj_weights_sized<DT, ODT, 128>(p, vec, st) : pj_weights_sized<DT, ODT, 64>(p, vec, st);
+}
+
+// A type's rows and weights products; defined in kernels_project_{f32,bf16,f16}.hip.
+#define PJ_DEFINE(NAME, DT)                                                                            \
+    hipError_t launch_proj_rows_##NAME(const ProjRows& p, hipStream_t st) {                            \
+        return p.out_dtype == VDB_F32 ? pj_rows<DT, VDB_F32>(p, st) : pj_rows<DT, DT>(p, st);          \
+    }                                                                                                  \
+    hipError_t launch_proj_weights_##NAME(const ProjWeights& p, hipStream_t st) {                      \
+        return p.out_dtype == VDB_F32 ? pj_weights<DT, VDB_F32>(p, st) : pj_weights<DT, DT>(p, st);    \
+    }
+
+}  // namespace vdb

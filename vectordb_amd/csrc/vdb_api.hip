@@ -2089,12 +2089,22 @@ static bool blocks_overlap(const void* p, int64_t pb, const void* q, int64_t qb)
     return p && q && pb > 0 && qb > 0 && (uintptr_t)p < (uintptr_t)q + (uintptr_t)qb && (uintptr_t)q < (uintptr_t)p + (uintptr_t)pb;
 }
 
-static int64_t proj_intermediate_bytes(const vdb_projection* p, int64_t n) {
-    return (int64_t)round_up((size_t)n * proj_rank_pad(p->rank) * sizeof(float), 256);
-}
+// Workspace of an adapted call over n rows: the parts of the low-rank intermediate that the output takes up, their row
+// scales, and, backward, both intermediates in fp32 for the factors' gradients.
+struct ProjWork {
+    int64_t parts, scale, f32, all;
+    int rp32;
+    ProjWork(const vdb_projection* p, int64_t n, bool backward) {
+        rp32 = proj_rank_pad(p->rank, VDB_F32);
+        parts = (int64_t)round_up((size_t)n * proj_parts(p->dtype) * proj_rank_pad(p->rank, p->dtype) * (p->dtype == VDB_F32 ? 4 : 2), 256);
+        scale = p->dtype == VDB_F16 ? (int64_t)round_up((size_t)n * 4, 256) : 0;
+        f32 = backward ? (int64_t)round_up((size_t)n * rp32 * 4, 256) : 0;
+        all = parts + scale + 2 * f32;
+    }
+};
 
 static int64_t proj_workspace(const vdb_projection* p, int64_t n, bool adapted, bool backward) {
-    return adapted ? proj_intermediate_bytes(p, n) * (backward ? 2 : 1) : 0;
+    return adapted ? ProjWork(p, n, backward).all : 0;
 }
 
 static int workspace_check(void* ws, int64_t have, int64_t want) {
@@ -2121,16 +2131,17 @@ static ProjRows proj_forward(const vdb_projection* p, int64_t n, const void* x, 
 
 // h = s x A^T, then y = x W^T + h B^T
 static hipError_t proj_adapted(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets, const int32_t* ids,
-                               int64_t requests, void* y, int64_t ldy, int out_dtype, float* h, hipStream_t st) {
+                               int64_t requests, void* y, int64_t ldy, int out_dtype, void* ws, hipStream_t st) {
+    const ProjWork wk(p, n, false);
     ProjShrink s{};
     s.x = x; s.ldx = ldx; s.n = n; s.K = (int)p->dim_in; s.dtype = p->dtype;
     s.f = p->a; s.f_adapter = p->rank * p->dim_in; s.f_rank = p->dim_in; s.f_k = 1;
-    s.scale = p->scale; s.h = h; s.rank = p->rank; s.rp = proj_rank_pad(p->rank);
+    s.scale = p->scale; s.rank = p->rank; s.h = ws; s.h_scale = (float*)((char*)ws + wk.parts);
     s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = ids; s.adapters = p->adapters;
     hipError_t e = launch_proj_shrink(s, st);
     if (e != hipSuccess) return e;
     ProjRows r = proj_forward(p, n, x, ldx, offsets, requests, y, ldy, out_dtype);
-    r.w_group = 0; r.ids = ids; r.adapters = p->adapters; r.h = h; r.rp = s.rp; r.rank = p->rank;
+    r.w_group = 0; r.ids = ids; r.adapters = p->adapters; r.h = s.h; r.h_scale = s.h_scale; r.rank = p->rank;
     r.f = p->b; r.f_adapter = p->dim_out * p->rank; r.f_col = p->rank; r.f_rank = 1;
     return launch_proj_rows(r, st);
 }
@@ -2216,7 +2227,7 @@ int vdb_project_adapted_dev(const vdb_projection* p, int64_t n, const void* x, i
     }
     if ((rc = enter())) return rc;
     if (n == 0 || requests == 0) return VDB_OK;
-    VDB_HIP(proj_adapted(p, n, x, ldx, offsets, adapter_ids, requests, y, ldy, p->out_dtype, (float*)workspace, (hipStream_t)stream));
+    VDB_HIP(proj_adapted(p, n, x, ldx, offsets, adapter_ids, requests, y, ldy, p->out_dtype, workspace, (hipStream_t)stream));
     return VDB_OK;
 }
 
@@ -2227,7 +2238,8 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     if (rc) return rc;
     if (!da != !db) return fail(VDB_EINVAL, "da and db come together");
     if (!dx && !da) return fail(VDB_EINVAL, "dx, da and db are all null");
-    const int64_t want = proj_workspace(p, n, true, true), half = proj_intermediate_bytes(p, n);
+    const ProjWork wk(p, n, true);
+    const int64_t want = wk.all;
     const RowsArg rdy{dy, lddy, p->dim_out, p->dtype, "dy"}, rx{x, ldx, p->dim_in, p->dtype, "x"}, rdx{dx, lddx, p->dim_in, p->out_dtype, "dx"};
     const int64_t oe = p->out_dtype == VDB_F32 ? 4 : 2, pairs = (int64_t)p->adapters * p->rank, e = rx.esize();
     const int64_t dab = pairs * p->dim_in * oe, dbb = pairs * p->dim_out * oe;
@@ -2255,36 +2267,38 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     }
     if ((rc = enter())) return rc;
     hipStream_t st = (hipStream_t)stream;
-    float* const h = (float*)workspace;
-    float* const g = (float*)((char*)workspace + half);
-    const int rp = proj_rank_pad(p->rank);
+    char* const ws = (char*)workspace;
+    float* const g32 = (float*)(ws + wk.parts + wk.scale);
+    float* const h32 = (float*)(ws + wk.parts + wk.scale + wk.f32);
     ProjShrink s{};
-    s.n = n; s.dtype = p->dtype; s.scale = p->scale; s.rank = p->rank; s.rp = rp;
+    s.n = n; s.dtype = p->dtype; s.scale = p->scale; s.rank = p->rank; s.rp32 = wk.rp32;
     s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = adapter_ids; s.adapters = p->adapters;
     // g = s dy B
-    s.x = dy; s.ldx = lddy; s.K = (int)p->dim_out; s.h = g;
+    s.x = dy; s.ldx = lddy; s.K = (int)p->dim_out;
     s.f = p->b; s.f_adapter = p->dim_out * p->rank; s.f_rank = 1; s.f_k = p->rank;
+    s.h = dx ? ws : nullptr; s.h_scale = (float*)(ws + wk.parts); s.h32 = da ? g32 : nullptr;
     VDB_HIP(launch_proj_shrink(s, st));
     if (da) {
         // h = s x A^T, again rather than kept from the forward pass
-        s.x = x; s.ldx = ldx; s.K = (int)p->dim_in; s.h = h;
+        s.x = x; s.ldx = ldx; s.K = (int)p->dim_in;
         s.f = p->a; s.f_adapter = p->rank * p->dim_in; s.f_rank = p->dim_in; s.f_k = 1;
+        s.h = nullptr; s.h_scale = nullptr; s.h32 = h32;
         VDB_HIP(launch_proj_shrink(s, st));
     }
     if (dx && n > 0) {
         ProjRows r = proj_forward(p, n, dy, lddy, offsets, requests, dx, lddx, p->out_dtype);
         r.w_group = 0; r.w_by_k = true; r.N = (int)p->dim_in; r.K = (int)p->dim_out;
-        r.ids = adapter_ids; r.adapters = p->adapters; r.h = g; r.rp = rp; r.rank = p->rank;
+        r.ids = adapter_ids; r.adapters = p->adapters; r.h = ws; r.h_scale = (const float*)(ws + wk.parts); r.rank = p->rank;
         r.f = p->a; r.f_adapter = p->rank * p->dim_in; r.f_col = 1; r.f_rank = p->dim_in;
         VDB_HIP(launch_proj_rows(r, st));
     }
     if (da) {
         ProjFactor f{};
-        f.rp = rp; f.rank = p->rank; f.n = n; f.dtype = p->dtype; f.out_dtype = p->out_dtype;
+        f.rp = wk.rp32; f.rank = p->rank; f.n = n; f.dtype = p->dtype; f.out_dtype = p->out_dtype;
         f.offsets = (const long long*)offsets; f.segments = (int)requests; f.ids = adapter_ids; f.adapters = p->adapters;
-        f.h = g; f.x = x; f.ldx = ldx; f.N = (int)p->dim_in; f.out = da; f.by_col = false;
+        f.h = g32; f.x = x; f.ldx = ldx; f.N = (int)p->dim_in; f.out = da; f.by_col = false;
         VDB_HIP(launch_proj_factor(f, st));
-        f.h = h; f.x = dy; f.ldx = lddy; f.N = (int)p->dim_out; f.out = db; f.by_col = true;
+        f.h = h32; f.x = dy; f.ldx = lddy; f.N = (int)p->dim_out; f.out = db; f.by_col = true;
         VDB_HIP(launch_proj_factor(f, st));
     }
     return VDB_OK;
@@ -2352,7 +2366,7 @@ int vdb_search_projected_dev(const char* name, const vdb_projection* p, int64_t 
             float* const q = (float*)((char*)ws->proj.p + hb);
             hipError_t e = launch_proj_zero_outside(q, t->dim, nq, (const long long*)offsets, (int)requests, st);
             if (e == hipSuccess && requests > 0)
-                e = proj_adapted(p, nq, x, ldx, offsets, adapter_ids, requests, q, t->dim, VDB_F32, (float*)ws->proj.p, st);
+                e = proj_adapted(p, nq, x, ldx, offsets, adapter_ids, requests, q, t->dim, VDB_F32, ws->proj.p, st);
             if (e != hipSuccess) rc = fail(VDB_EHIP, std::string("projection: ") + hipGetErrorString(e));
             else {
                 std::shared_lock<std::shared_mutex> tl(t->mu);
