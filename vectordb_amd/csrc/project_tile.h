@@ -345,49 +345,155 @@ struct PJProduct {
     }
 };
 
-// Low-rank term of a wave's block, before the main product: for every request that meets 16 of its rows, h f^T, taken over
-// by the rows of that request only, so that what one adapter holds never reaches another request's rows.  The fp32
-// intermediate h comes in parts of the rows' type that add up to it (bf16: three; fp16: two, with a power of two for each row
-// that brings its largest entry to 1/2..1, as fp16 could not hold it; see pj_store_parts), so that the term runs on
-// the 16-bit matrix unit without rounding h.
-template <int DT, bool FV, int B>
-__device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, int colb, pj_f32x4 (&acc)[B][B]) {
+// ------------------------------------------------------------------------------------------- low-rank term
+// The term h f^T of a wave's block, before the main product.  The fp32 intermediate h comes in parts of the rows' type that add up
+// to it (bf16: three; fp16: two, with a power of two for each row that brings its largest entry to 1/2..1, as fp16 could
+// not hold it), so that neither way below rounds h:
+//   up to two adapters in 16 rows: the matrix unit, all 16 rows by one adapter, taken over by the rows of that adapter only,
+//     so that what one adapter holds never reaches another request's rows;
+//   more: every lane for itself, its row by its four columns, which waits once for all adapters instead of once for each.
+
+// Adapter of each of B times 16 rows (lane l: row + 16 i + l % 16); -1: none.
+template <int B>
+__device__ __forceinline__ void pj_row_adapters(const ProjRows& p, long long row, int (&am)[B]) {
+    const int li = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < B; ++i) am[i] = -1;
+    pj_each_request(p.offsets, p.ids, p.segments, p.adapters, p.n, row, row + B * 16, [&](long long b, long long e, int a) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const long long m = row + i * 16 + li;
+            am[i] = m >= b && m < e ? a : am[i];
+        }
+    });
+}
+
+// How the factor f lies: entry (column, rank) of an adapter at column * f_col + rank * f_rank elements (32 bits hold it).
+//   PJ_F_RANKS   ranks contiguous, 16-byte pieces of them aligned (B of a forward pass)
+//   PJ_F_COLS    columns contiguous, groups of four aligned and whole (A of a backward pass)
+//   PJ_F_ANY     neither
+enum { PJ_F_ANY = 0, PJ_F_RANKS = 1, PJ_F_COLS = 2 };
+
+// 16 rows by one adapter on the matrix unit; t: lane's row by columns colb + 16 j + 4 (l / 16) + 0..3
+template <int DT, int F, int C>
+__device__ __forceinline__ void pj_low_rank_block(const ProjRows& p, long long mc, int colb, int a, pj_f32x4 (&t)[C]) {
     typedef typename PJ<DT>::T T;
     constexpr int V = 16 / PJ<DT>::E, QS = 4 * V, NP = proj_parts(DT);
     const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
     const int rp = proj_rank_pad(p.rank, DT);
-    pj_each_request(p.offsets, p.ids, p.segments, p.adapters, p.n, row, row + B * 16, [&](long long b, long long e, int a) {
-        const T* f = (const T*)p.f + (long long)a * p.f_adapter;
+    const unsigned fr = (unsigned)p.f_rank, fcol = (unsigned)p.f_col;
+    const T* f = (const T*)p.f + (long long)a * p.f_adapter;
+    const T* h = (const T*)p.h + mc * (NP * rp);
+#pragma unroll 1
+    for (int q = 0; q < p.rank; q += QS) {
+        pj_u32x4 hv[NP];
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const long long r0 = row + i * 16, m = r0 + li;
-            if (b >= r0 + 16 || e <= r0) continue;
-            const T* h = (const T*)p.h + (m < p.n ? m : p.n - 1) * (NP * rp);
-            pj_f32x4 t[B] = {};
-            for (int q = 0; q < p.rank; q += QS) {
-                pj_u32x4 hv[NP];
+        for (int u = 0; u < NP; ++u) hv[u] = *(const pj_u32x4*)(h + u * rp + q + lh * V);
 #pragma unroll
-                for (int u = 0; u < NP; ++u) hv[u] = *(const pj_u32x4*)(h + u * rp + q + lh * V);
+        for (int j = 0; j < C; ++j) {
+            const int col = colb + j * 16 + li, r = q + lh * V;
+            const unsigned at = (unsigned)(col < p.N ? col : p.N - 1) * fcol + (unsigned)r * fr;
+            union { T t[V]; pj_u32x4 v; } fv;
+            if constexpr (F == PJ_F_RANKS) fv.v = *(const pj_u32x4*)(r < p.rank ? f + at : (const T*)pj_zero16);
+            else
 #pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    const int col = colb + j * 16 + li, r = q + lh * V;
-                    const T* fc = f + (long long)(col < p.N ? col : p.N - 1) * p.f_col;
+                for (int u = 0; u < V; ++u) fv.t[u] = r + u < p.rank ? f[at + (unsigned)u * fr] : (T)0;
+#pragma unroll
+            for (int u = NP - 1; u >= 0; --u) t[j] = pj_mfma<DT>(fv.v, hv[u], t[j]);
+            if constexpr (F != PJ_F_RANKS) asm volatile("" ::: "memory");       // one block's loads at a time: registers
+        }
+    }
+}
+
+// Every lane its own row's adapter: t += h[m] f[a]^T for its four columns of each block, ranks q0, q0 + qs, ... in steps of V
+template <int DT, int F, int C>
+__device__ __forceinline__ void pj_low_rank_lanes(const ProjRows& p, long long mc, int colb, int a, int q0, int qs, pj_f32x4 (&t)[C]) {
+    typedef typename PJ<DT>::T T;
+    typedef T tx4 __attribute__((ext_vector_type(4)));
+    constexpr int V = 16 / PJ<DT>::E, NP = proj_parts(DT);
+    const int lh = (threadIdx.x & 63) >> 4;
+    const int rp = proj_rank_pad(p.rank, DT);
+    const unsigned fr = (unsigned)p.f_rank, fcol = (unsigned)p.f_col;
+    const T* f = (const T*)p.f + (long long)(a < 0 ? 0 : a) * p.f_adapter;
+    const T* h = (const T*)p.h + mc * (NP * rp);
+#pragma unroll 1
+    for (int q = q0; q < p.rank; q += qs) {
+        float hq[V] = {};
+#pragma unroll
+        for (int u = NP - 1; u >= 0; --u) {
+            union { T t[V]; pj_u32x4 v; } hv;
+            hv.v = *(const pj_u32x4*)(h + u * rp + q);
+#pragma unroll
+            for (int k = 0; k < V; ++k) hq[k] += pj_to_f32<DT>(hv.t[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int col = colb + j * 16 + lh * 4;
+            if constexpr (F == PJ_F_COLS) {
+                const unsigned at = (unsigned)(col < p.N ? col : p.N - 4) * fcol + (unsigned)q * fr;
+                tx4 fv[V];
+#pragma unroll
+                for (int k = 0; k < V; ++k) fv[k] = *(const tx4*)(q + k < p.rank ? f + at + (unsigned)k * fr : (const T*)pj_zero16);
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) t[j][n] = __builtin_fmaf(hq[k], pj_to_f32<DT>(fv[k][n]), t[j][n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const unsigned at = (unsigned)(col + n < p.N ? col + n : p.N - 1) * fcol + (unsigned)q * fr;
                     union { T t[V]; pj_u32x4 v; } fv;
-                    if constexpr (FV) fv.v = *(const pj_u32x4*)(r < p.rank ? fc + r : (const T*)pj_zero16);
+                    if constexpr (F == PJ_F_RANKS) fv.v = *(const pj_u32x4*)(f + at);
                     else
 #pragma unroll
-                        for (int u = 0; u < V; ++u) fv.t[u] = r + u < p.rank ? fc[(long long)(r + u) * p.f_rank] : (T)0;
+                        for (int k = 0; k < V; ++k) fv.t[k] = q + k < p.rank ? f[at + (unsigned)k * fr] : (T)0;
 #pragma unroll
-                    for (int u = NP - 1; u >= 0; --u) t[j] = pj_mfma<DT>(fv.v, hv[u], t[j]);
+                    for (int k = 0; k < V; ++k) t[j][n] = __builtin_fmaf(hq[k], pj_to_f32<DT>(fv.t[k]), t[j][n]);
                 }
             }
-            if (m >= b && m < e) {
-                const float sc = DT == VDB_F16 ? p.h_scale[m] : 1.f;
-#pragma unroll
-                for (int j = 0; j < B; ++j) acc[i][j] = DT == VDB_F16 ? t[j] * sc : t[j];
-            }
+            if constexpr (F != PJ_F_RANKS) asm volatile("" ::: "memory");
         }
-    });
+    }
+}
+
+// B blocks of 16 rows from `row`, C of 16 columns from `colb`.  `waves` > 1: that many waves share the block, and the sum of
+// their accumulators is the term.
+template <int DT, int F, int B, int C>
+__device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, int colb, pj_f32x4 (&acc)[B][C], int waves = 1, int wave = 0) {
+    constexpr int V = 16 / PJ<DT>::E;
+    const int li = threadIdx.x & 15;
+    int am[B];
+    pj_row_adapters<B>(p, row, am);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const long long m = row + i * 16 + li, mc = m < p.n ? m : p.n - 1;
+        unsigned left = (unsigned)__ballot(am[i] >= 0) & 0xffffu;
+        if (!left) continue;
+        const int a0 = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
+        left &= ~(unsigned)__ballot(am[i] == a0);
+        int a1 = -1;
+        if (left) {
+            a1 = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
+            left &= ~(unsigned)__ballot(am[i] == a1);
+        }
+        pj_f32x4 t[C] = {};
+        if (!left) {
+            if (wave == 0) pj_low_rank_block<DT, F, C>(p, mc, colb, a0, t);
+            if (a1 >= 0) {
+                pj_f32x4 t1[C] = {};
+                if (wave == waves - 1) pj_low_rank_block<DT, F, C>(p, mc, colb, a1, t1);
+#pragma unroll
+                for (int j = 0; j < C; ++j) if (am[i] == a1) t[j] = t1[j];
+            }
+        } else {
+            pj_low_rank_lanes<DT, F, C>(p, mc, colb, am[i], wave * V, waves * V, t);
+        }
+        if (am[i] >= 0) {
+            const float sc = DT == VDB_F16 ? p.h_scale[mc] : 1.f;
+#pragma unroll
+            for (int j = 0; j < C; ++j) acc[i][j] = DT == VDB_F16 ? t[j] * sc : t[j];
+        }
+    }
 }
 
 struct PJRowsArgs {
@@ -396,7 +502,7 @@ struct PJRowsArgs {
     bool vec_out;
 };
 
-template <int DT, int ODT, bool NK, bool VEC, bool ADAPT, bool FV, int R>
+template <int DT, int ODT, bool NK, bool VEC, bool ADAPT, int F, int R>
 __global__ void __launch_bounds__(PJ_THREADS, 2)
 proj_rows_kernel(PJRowsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char pj_lds[];
@@ -427,7 +533,7 @@ proj_rows_kernel(PJRowsArgs a) {
     prod.om.init((const T*)p.x, p.ldx, row0, row1);
     prod.on.init((const T*)p.w + (long long)seg * p.w_group, p.ldw, col0, p.N);
     prod.begin(p.K, pj_lds);
-    if constexpr (ADAPT) pj_low_rank<DT, FV, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), acc);
+    if constexpr (ADAPT) pj_low_rank<DT, F, B, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), acc);
     prod.run(pj_lds, wm, wn, acc);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -439,6 +545,63 @@ proj_rows_kernel(PJRowsArgs a) {
             if (c < p.N) pj_store4<ODT>(p.y, m * p.ldy + c, acc[i][j], p.N - c, a.vec_out);
         }
     }
+}
+
+// A few rows: 16 rows x 16 columns per workgroup, so that the matrix is read by many CUs; the four waves take every fourth step
+// of the contracted axis, straight from memory into fragments with all loads of U steps ahead of the products, and add up
+// through LDS in wave order.  The requests of the low-rank term are divided among the waves as well.
+template <int DT, int ODT, bool NK, bool VEC, bool ADAPT, int F>
+__global__ void __launch_bounds__(PJ_THREADS)
+proj_few_kernel(PJRowsArgs a) {
+    typedef typename PJ<DT>::T T;
+    constexpr int V = 16 / PJ<DT>::E, KS = 4 * V, U = 4;
+    __shared__ pj_f32x4 part[3][64];
+    const ProjRows& p = a.p;
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    long long row0, row1, first = 0;
+    int seg = 0, col;
+    if constexpr (ADAPT) {
+        col = blockIdx.x % a.col_tiles;
+        row0 = (long long)(blockIdx.x / a.col_tiles) * 16;
+        first = pj_clamp(p.offsets[0], p.n); row1 = pj_clamp(p.offsets[p.segments], p.n);
+        if (row0 >= row1 || row0 + 16 <= first) return;
+    } else {
+        if (!pj_find_tile(p.offsets, p.segments, p.n, 16, a.col_tiles, blockIdx.x, seg, row0, row1, col)) return;
+    }
+    const long long m = row0 + li;
+    const int c = col * 16 + li;
+    const T* x = (const T*)p.x + (m < row1 ? m : row1 - 1) * p.ldx;
+    const T* w = (const T*)p.w + (long long)seg * p.w_group + (NK ? (c < p.N ? c : p.N - 1) : (long long)(c < p.N ? c : p.N - 1) * p.ldw);
+    pj_f32x4 acc[1][1] = {};
+    if constexpr (ADAPT) pj_low_rank<DT, F, 1, 1>(p, row0, col * 16, acc, 4, wave);
+    for (int k0 = wave * KS; k0 < p.K; k0 += U * 4 * KS) {
+        union frag { T t[V]; pj_u32x4 v; } xa[U], wa[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 4 * KS + lh * V;
+            if constexpr (VEC) xa[u].v = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
+            else
+#pragma unroll
+                for (int j = 0; j < V; ++j) xa[u].t[j] = k + j < p.K ? x[k + j] : (T)0;
+            if constexpr (VEC && !NK) wa[u].v = *(const pj_u32x4*)(k < p.K ? w + k : (const T*)pj_zero16);
+            else
+#pragma unroll
+                for (int j = 0; j < V; ++j) wa[u].t[j] = k + j < p.K ? w[NK ? (k + j) * p.ldw : (long long)(k + j)] : (T)0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc[0][0] = pj_mfma<DT>(wa[u].v, xa[u].v, acc[0][0]);
+    }
+    if (wave) part[wave - 1][lane] = acc[0][0];
+    __syncthreads();
+    if (wave) return;
+    pj_f32x4 v = acc[0][0];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += part[i][lane][j];
+    const int cs = col * 16 + lh * 4;
+    if (m < row1 && m >= first && cs < p.N) pj_store4<ODT>(p.y, m * p.ldy + cs, v, p.N - cs, a.vec_out);
 }
 
 struct PJWeightsArgs {
@@ -491,6 +654,13 @@ static hipError_t pj_launch(K kernel, dim3 grid, size_t lds, const A& args, hipS
 // 64 x 64 tiles where 128 x 128 ones would leave CUs without work.
 static inline bool pj_small_tiles(long long tiles128) { return tiles128 < 256; }
 
+// The low-rank factor can be read in vectors: forward its ranks are contiguous, backward its columns.
+template <int DT, int V> static bool pj_factor_vec(const ProjRows& p) {
+    if (!p.ids) return false;
+    return p.f_rank == 1 ? p.rank % V == 0 && (uintptr_t)p.f % 16 == 0
+                         : p.N % 4 == 0 && (uintptr_t)p.f % (4 * PJ<DT>::E) == 0;
+}
+
 template <int DT, int ODT, int R>
 static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     PJRowsArgs a;
@@ -501,14 +671,19 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     const long long row_tiles = p.ids ? (p.n + R - 1) / R : p.n / R + p.segments;
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const size_t lds = PJRing<R>::BYTES;
-    // low-rank factor: forward its ranks are contiguous, backward its columns
-    const bool fv = p.ids && p.f_rank == 1 && p.rank % V == 0 && (uintptr_t)p.f % 16 == 0;
+    const bool fv = pj_factor_vec<DT, V>(p);
 #define PJ_ROWS(NK, VEC)                                                                              \
-    (!p.ids ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, false, R>, grid, lds, a, st)        \
-     : fv   ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, !NK, R>, grid, lds, a, st)           \
-            : pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, false, R>, grid, lds, a, st))
-    if constexpr (R == 128) return p.w_by_k ? PJ_ROWS(true, true) : PJ_ROWS(false, true);
-    else {
+    (!p.ids ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY, R>, grid, lds, a, st)     \
+     : fv   ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st) \
+            : pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, PJ_F_ANY, R>, grid, lds, a, st))
+    if constexpr (R == 128) {
+        // (a factor that cannot be read in vectors would spill here)
+#define PJ_BIG(NK)                                                                                                        \
+    (p.ids ? pj_launch(proj_rows_kernel<DT, ODT, NK, true, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st)       \
+           : pj_launch(proj_rows_kernel<DT, ODT, NK, true, false, PJ_F_ANY, R>, grid, lds, a, st))
+        return p.w_by_k ? PJ_BIG(true) : PJ_BIG(false);
+#undef PJ_BIG
+    } else {
         if (p.w_by_k) return vec ? PJ_ROWS(true, true) : PJ_ROWS(true, false);
         return vec ? PJ_ROWS(false, true) : PJ_ROWS(false, false);
     }
@@ -516,12 +691,38 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
 }
 
 template <int DT, int ODT>
+static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
+    PJRowsArgs a;
+    a.p = p;
+    a.col_tiles = (p.N + 15) / 16;
+    constexpr int V = 16 / PJ<DT>::E;
+    a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 4 * PJ<ODT>::E);
+    const long long row_tiles = p.ids ? (p.n + 15) / 16 : p.n / 16 + p.segments;
+    const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
+    const bool fv = pj_factor_vec<DT, V>(p);
+#define PJ_FEW(NK, VEC)                                                                          \
+    (!p.ids ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY>, grid, 0, a, st)      \
+     : fv   ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, true, NK ? PJ_F_COLS : PJ_F_RANKS>, grid, 0, a, st) \
+            : pj_launch(proj_few_kernel<DT, ODT, NK, VEC, true, PJ_F_ANY>, grid, 0, a, st))
+    if (p.w_by_k) return vec ? PJ_FEW(true, true) : PJ_FEW(true, false);
+    return vec ? PJ_FEW(false, true) : PJ_FEW(false, false);
+#undef PJ_FEW
+}
+
+// Largest number of 64 x 64 tiles that is left to the kernel for a few rows.
+#ifndef PJ_FEW_TILES
+#define PJ_FEW_TILES 64
+#endif
+template <int DT, int ODT>
 static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool vec = pj_aligned(p.x, p.ldx, E, 16) && pj_aligned(p.w, p.ldw, E, 16) && p.w_group % V == 0 &&
                      p.K % V == 0 && (!p.w_by_k || p.N % V == 0);
     const long long tiles = ((p.n + 127) / 128 + (p.ids ? 0 : p.segments / 2)) * ((p.N + 127) / 128);
-    return vec && !pj_small_tiles(tiles) ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
+    const long long tiles64 = ((p.n + 63) / 64) * ((p.N + 63) / 64);
+    if (tiles64 <= PJ_FEW_TILES) return pj_few<DT, ODT>(p, vec, st);
+    const bool big = vec && !pj_small_tiles(tiles) && (!p.ids || pj_factor_vec<DT, V>(p));
+    return big ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
 }
 
 template <int DT, int ODT, int R>
