@@ -29,102 +29,238 @@ __device__ __forceinline__ void pj_store_parts(const ProjShrink& p, long long m,
     }
 }
 
+// How the factor of a shrink lies: FK: contiguous along the contracted axis, 16-byte pieces aligned (A of a forward pass);
+// FR: contiguous along the ranks, whole 16-byte pieces (B of a backward pass); else any strides.
+enum { PJ_S_ANY = 0, PJ_S_FK = 1, PJ_S_FR = 2 };
+
+// The rows' side of XS steps of the contracted axis at k0, k0 + stride, ...
+template <int DT, int XS, bool XV>
+__device__ __forceinline__ void pj_shrink_load_x(const ProjShrink& p, const typename PJ<DT>::T* x, int k0, int stride, pj_u32x4 (&xa)[XS]) {
+    typedef typename PJ<DT>::T T;
+    constexpr int V = 16 / PJ<DT>::E;
+    const int lh = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int u = 0; u < XS; ++u) {
+        const int k = k0 + u * stride + lh * V;
+        union { T t[V]; pj_u32x4 v; } f;
+        if constexpr (XV) f.v = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
+        else
+#pragma unroll
+            for (int j = 0; j < V; ++j) f.t[j] = k + j < p.K ? x[k + j] : (T)0;
+        xa[u] = f.v;
+    }
+}
+
+// U steps: acc[i] += (ranks 16 i.. of f) x^T, all loads ahead of the products.
+// FR, 16-bit: a step's 32 lines of the factor pass through `lds`, a part of it that belongs to this wave, and come back
+// transposed (ds_read_b64_tr_b16: blocks of 4 lines x 16 ranks).
+template <int DT, int NRB, int F, int U>
+__device__ __forceinline__ void pj_shrink_steps(const ProjShrink& p, const pj_u32x4* xa, const typename PJ<DT>::T* f, int k0, int stride,
+                                                char* lds, pj_f32x4 (&acc)[NRB]) {
+    typedef typename PJ<DT>::T T;
+    constexpr int V = 16 / PJ<DT>::E;
+    constexpr bool TR = F == PJ_S_FR && DT != VDB_F32;
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    union frag { T t[V]; pj_u32x4 v; } fa[U][NRB];
+    const unsigned fr = (unsigned)p.f_rank, fk = (unsigned)p.f_k;            // an adapter's elements number less than 2^32
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * stride + lh * V;
+        if constexpr (TR) {
+            // pieces of 8 ranks: piece c is line c / (rank / 8) of the step
+            const int ppl = p.rank / 8, kb = k0 + u * stride;
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                const int c = i * 64 + lane;
+                const bool in = c < 32 * ppl && kb + c / ppl < p.K;
+                fa[u][i].v = *(const pj_u32x4*)(in ? f + (unsigned)kb * fk + (unsigned)c * 8u : (const T*)pj_zero16);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                const int q = i * 16 + li;
+                const unsigned at = (unsigned)q * fr + (unsigned)k * fk;
+                if constexpr (F == PJ_S_FK) fa[u][i].v = *(const pj_u32x4*)(k < p.K && q < p.rank ? f + at : (const T*)pj_zero16);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; ++j) fa[u][i].t[j] = k + j < p.K && q < p.rank ? f[at + (unsigned)j * fk] : (T)0;
+            }
+        }
+    }
+    if constexpr (TR) {
+        const int line = p.rank * 2;                   // bytes; ranks past the last read the next line and are dropped by the caller
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) *(pj_u32x4*)(lds + (u * NRB + i) * 1024 + lane * 16) = fa[u][i].v;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                const char* at = lds + u * NRB * 1024 + (lh * 8 + (li >> 2)) * line + i * 32 + (li & 3) * 8;
+                union { pj_s16x4 h[2]; pj_u32x4 v; } t;
+                t.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PJ_LOCAL pj_s16x4*)at);
+                t.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PJ_LOCAL pj_s16x4*)(at + 4 * line));
+                fa[u][i].v = t.v;
+            }
+        __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) acc[i] = pj_mfma<DT>(fa[u][i].v, xa[u], acc[i]);      // lane: row, ranks 16 i + 4 lh + 0..3
+}
+
+// LDS of a wave for pj_shrink_steps: the lines of U steps, and what the reads of ranks past the last may touch behind them
+template <int DT, int NRB, int F, int U> constexpr int pj_shrink_lds() { return F == PJ_S_FR && DT != VDB_F32 ? U * NRB * 1024 + 256 : 16; }
+
+// Scales one row block's sums and stores the rows of adapter `ad` (`mine`: this lane's row is one of them).
+template <int DT, int NRB>
+__device__ __forceinline__ void pj_shrink_store(const ProjShrink& p, long long m, bool mine, int ad, pj_f32x4 (&acc)[NRB]) {
+    const int lh = (threadIdx.x & 63) >> 4, rp = proj_rank_pad(p.rank, DT);
+    const float sc = p.scale ? p.scale[ad] : 1.f;
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < NRB; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[i][j] = i * 16 + lh * 4 + j < p.rank ? sc * acc[i][j] : 0.f;
+            const float size = fabsf(acc[i][j]);
+            if (size < __builtin_huge_valf()) most = fmaxf(most, size);
+        }
+    float down = 1.f;
+    if constexpr (DT == VDB_F16) {
+        // a power of two that brings the row's largest finite entry to 1/2..1 (1 where that entry is next to the limits of fp32)
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const int ex = (int)(__float_as_uint(most) >> 23);
+        const bool scaled = ex > 2 && ex < 253;
+        down = scaled ? __uint_as_float((unsigned)(253 - ex) << 23) : 1.f;      // 2^(126 - ex)
+        if (p.h_scale && lh == 0 && mine) p.h_scale[m] = scaled ? __uint_as_float((unsigned)(ex + 1) << 23) : 1.f;
+    }
+    if (mine) {
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) if (i * 16 < rp) pj_store_parts<DT>(p, m, i * 16 + lh * 4, rp, acc[i], down);
+    }
+}
+
+// Adapter of each of B times 16 rows (lane l: row + 16 i + l % 16); -1: none.
+template <int B>
+__device__ __forceinline__ void pj_row_adapters(const ProjShrink& p, long long row, int (&am)[B]) {
+    const int li = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < B; ++i) am[i] = -1;
+    pj_each_request(p.offsets, p.ids, p.segments, p.adapters, p.n, row, row + B * 16, [&](long long b, long long e, int a) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const long long m = row + i * 16 + li;
+            am[i] = m >= b && m < e ? a : am[i];
+        }
+    });
+}
+
 // h = s x f^T for 16 rows: the four waves take every fourth step of the contracted axis and add up through LDS in wave
-// order.  Each request that meets the 16 rows is multiplied on its own and keeps its own rows; where requests are shorter than
-// that, `share` workgroups divide the requests of a block of rows among them.
-template <int DT, int NRB, bool XV, bool FV>
+// order.  Each adapter that the 16 rows meet is multiplied on its own and keeps its own rows; `share` workgroups divide
+// the adapters of a block of rows among them.  The rows are loaded before the adapters are known.
+// What bounds it is latency (offsets, then the factor, then the exchange): a wave to 16 rows without the exchange, and 64 rows
+// to a workgroup, which reads the factor a quarter as often, were both slower (56 and 45 against 47 us for 32 768 x 1024 rows of
+// rank 64, 24 and 26 against 18 us for 16 384 x 768 of rank 16).
+template <int DT, int NRB, bool XV, int F>
 __global__ void __launch_bounds__(256)
 proj_shrink_kernel(ProjShrink p, int share) {
     typedef typename PJ<DT>::T T;
-    constexpr int V = 16 / PJ<DT>::E, KS = 4 * V;          // elements per lane and per step
-    constexpr int U = NRB <= 2 ? 4 : 2;
+    constexpr int KS = 64 / PJ<DT>::E, XS = 8, U = NRB <= 2 ? 4 : 2;
     __shared__ pj_f32x4 part[3][NRB][64];
-    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4, wave = threadIdx.x >> 6;
+    __shared__ __attribute__((aligned(16))) char lds[4][pj_shrink_lds<DT, NRB, F, U>()];
+    const int lane = threadIdx.x & 63, li = lane & 15, wave = threadIdx.x >> 6;
     const long long r0 = (long long)(blockIdx.x / share) * 16, m = r0 + li;
     const int mine = blockIdx.x % share;
-    const int rp = proj_rank_pad(p.rank, DT);
     const T* x = (const T*)p.x + (m < p.n ? m : p.n - 1) * p.ldx;
-    int turn = 0;
-    pj_each_request(p.offsets, p.ids, p.segments, p.adapters, p.n, r0, r0 + 16, [&](long long b, long long e, int ad) {
-        if (turn++ % share != mine) return;
+    pj_u32x4 xa[XS];
+    pj_shrink_load_x<DT, XS, XV>(p, x, wave * KS, 4 * KS, xa);
+    int am[1];
+    pj_row_adapters<1>(p, r0, am);
+    if (p.row_adapter && mine == 0 && wave == 0 && lane < 16 && m < p.n) p.row_adapter[m] = am[0];
+    unsigned left = (unsigned)__ballot(am[0] >= 0) & 0xffffu;
+    for (int turn = 0; left; turn = turn + 1 == share ? 0 : turn + 1) {
+        const int ad = __builtin_amdgcn_readlane(am[0], __builtin_ctz(left));
+        left &= ~(unsigned)__ballot(am[0] == ad);
+        if (turn != mine) continue;
         const T* f = (const T*)p.f + (long long)ad * p.f_adapter;
         pj_f32x4 acc[NRB] = {};
-        // U steps at a time, all their loads before the first product
-        for (int k0 = wave * KS; k0 < p.K; k0 += U * 4 * KS) {
-            union frag { T t[V]; pj_u32x4 v; } xa[U], fa[U][NRB];
+        for (int kc = wave * KS; kc < p.K; kc += XS * 4 * KS) {
+            if (p.K > XS * 4 * KS) pj_shrink_load_x<DT, XS, XV>(p, x, kc, 4 * KS, xa);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = k0 + u * 4 * KS + lh * V;
-                if constexpr (XV) xa[u].v = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
-                else
-#pragma unroll
-                    for (int j = 0; j < V; ++j) xa[u].t[j] = k + j < p.K ? x[k + j] : (T)0;
-#pragma unroll
-                for (int i = 0; i < NRB; ++i) {
-                    const int q = i * 16 + li;
-                    if constexpr (FV) fa[u][i].v = *(const pj_u32x4*)(k < p.K && q < p.rank ? f + (long long)q * p.f_rank + k : (const T*)pj_zero16);
-                    else
-#pragma unroll
-                        for (int j = 0; j < V; ++j)
-                            fa[u][i].t[j] = k + j < p.K && q < p.rank ? f[(long long)q * p.f_rank + (long long)(k + j) * p.f_k] : (T)0;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int i = 0; i < NRB; ++i) acc[i] = pj_mfma<DT>(fa[u][i].v, xa[u].v, acc[i]);      // lane: row m, ranks 16 i + 4 lh + 0..3
+            for (int u = 0; u < XS; u += U)
+                if (kc + u * 4 * KS < p.K) pj_shrink_steps<DT, NRB, F, U>(p, xa + u, f, kc + u * 4 * KS, 4 * KS, lds[wave], acc);
         }
         __syncthreads();
         if (wave)
 #pragma unroll
             for (int i = 0; i < NRB; ++i) part[wave - 1][i][lane] = acc[i];
         __syncthreads();
-        if (wave == 0) {
-            const float sc = p.scale ? p.scale[ad] : 1.f;
-            float most = 0.f;
+        if (wave) continue;
 #pragma unroll
-            for (int i = 0; i < NRB; ++i)
+        for (int i = 0; i < NRB; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v = acc[i][j];
+            for (int w = 0; w < 3; ++w)
 #pragma unroll
-                    for (int w = 0; w < 3; ++w) v += part[w][i][lane][j];
-                    acc[i][j] = i * 16 + lh * 4 + j < p.rank ? sc * v : 0.f;
-                    const float size = fabsf(acc[i][j]);
-                    if (size < __builtin_huge_valf()) most = fmaxf(most, size);
-                }
-            float down = 1.f;
-            if constexpr (DT == VDB_F16) {
-                // a power of two that brings the row's largest finite entry to 1/2..1 (1 where that entry is next to the limits of fp32)
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const int ex = (int)(__float_as_uint(most) >> 23);
-                const bool scaled = ex > 2 && ex < 253;
-                down = scaled ? __uint_as_float((unsigned)(253 - ex) << 23) : 1.f;      // 2^(126 - ex)
-                if (p.h_scale && lh == 0 && m >= b && m < e) p.h_scale[m] = scaled ? __uint_as_float((unsigned)(ex + 1) << 23) : 1.f;
-            }
-            if (m >= b && m < e) {
-#pragma unroll
-                for (int i = 0; i < NRB; ++i) if (i * 16 < rp) pj_store_parts<DT>(p, m, i * 16 + lh * 4, rp, acc[i], down);
-            }
-        }
-    });
+                for (int j = 0; j < 4; ++j) acc[i][j] += part[w][i][lane][j];
+        pj_shrink_store<DT, NRB>(p, m, am[0] == ad, ad, acc);
+    }
 }
 
 // ------------------------------------------------------------------------------------------- gradient of the factors
-// One adapter's [rank] x 64 columns: the four waves take its rows 16 at a time in turn, over every request that names the
+// One adapter's [rank] x 64 columns: the eight waves take its rows 16 at a time in turn, over every request that names the
 // adapter, and add up in wave order.  Products on the fp32 matrix unit: h is fp32, x is widened.
 // Lane l loads columns 4 (l % 16) + 0..3 of a row, so that product j of a step holds columns j, 4 + j, 8 + j, ...
-template <int DT, int ODT, int NRB, bool XV>
-__global__ void __launch_bounds__(256)
-proj_factor_kernel(ProjFactor p) {
+// The rows of the next turn are loaded while the current ones are multiplied.
+constexpr int PJ_FACTOR_WAVES = 8;
+
+template <int DT, int NRB, bool XV> struct PJFactorRows {
     typedef typename PJ<DT>::T T;
+    typedef T tx4 __attribute__((ext_vector_type(4)));
+    tx4 x[4];
+    float h[4][NRB];
+    __device__ __forceinline__ void load(const ProjFactor& p, long long r, long long e, int c0) {
+        const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const long long i = r + u * 4 + lh;
+            const bool ok = i < e;
+            const T* px = (const T*)p.x + (ok ? i : 0) * p.ldx + c0;
+            if constexpr (XV) x[u] = *(const tx4*)(ok && c0 < p.N ? px : (const T*)pj_zero16);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[u][j] = ok && c0 + j < p.N ? px[j] : (T)0;
+#pragma unroll
+            for (int q = 0; q < NRB; ++q) h[u][q] = ok && q * 16 < p.rp ? p.h[i * p.rp + q * 16 + li] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void multiply(pj_f32x4 (&acc)[NRB][4]) const {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < NRB; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[q][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(pj_to_f32<DT>(x[u][j]), h[u][q], acc[q][j], 0, 0, 0);
+    }
+};
+
+template <int DT, int ODT, int NRB, bool XV>
+__global__ void __launch_bounds__(PJ_FACTOR_WAVES * 64)
+proj_factor_kernel(ProjFactor p) {
     typedef typename PJ<ODT>::T O;
-    __shared__ pj_f32x4 part[3][4][64];
+    constexpr int W = PJ_FACTOR_WAVES;
+    __shared__ pj_f32x4 part[W - 1][4][64];
     const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4, wave = threadIdx.x >> 6;
     const int n0 = blockIdx.x * 64, ad = blockIdx.y, c0 = n0 + li * 4;
     pj_f32x4 acc[NRB][4] = {};
+    PJFactorRows<DT, NRB, XV> rows[2];
     int turn = 0;                          // blocks of 16 rows met so far
+    bool held = false;                     // rows[0] holds a block that has not been multiplied
     for (int s0 = 0; s0 < p.segments; s0 += 64) {
         const bool hit = s0 + lane < p.segments && p.ids[s0 + lane] == ad;
         unsigned long long mask = __ballot(hit);
@@ -132,33 +268,19 @@ proj_factor_kernel(ProjFactor p) {
             const int s = s0 + __builtin_ctzll(mask);
             mask &= mask - 1;
             const long long b = pj_clamp(p.offsets[s], p.n), e = pj_clamp(p.offsets[s + 1], p.n);
-            for (long long r = b; r < e; r += 16) {
-                if ((turn++ & 3) != wave) continue;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const long long i = r + u * 4 + lh;
-                    const bool ok = i < e;
-                    float xv[4];
-                    if constexpr (XV) {
-                        typedef T tx4 __attribute__((ext_vector_type(4)));
-                        const tx4 v = *(const tx4*)(ok && c0 < p.N ? (const T*)p.x + i * p.ldx + c0 : (const T*)pj_zero16);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) xv[j] = pj_to_f32<DT>(v[j]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) xv[j] = ok && c0 + j < p.N ? pj_to_f32<DT>(((const T*)p.x)[i * p.ldx + c0 + j]) : 0.f;
-                    }
-#pragma unroll
-                    for (int q = 0; q < NRB; ++q) {
-                        const float hv = ok && q * 16 < p.rp ? p.h[i * p.rp + q * 16 + li] : 0.f;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[q][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[j], hv, acc[q][j], 0, 0, 0);
-                    }
-                }
+            if (e <= b) continue;
+            const long long blocks = (e - b + 15) / 16;
+            const int start = (wave - turn % W + W) % W;         // this wave's first block of the request
+            turn = (int)((turn + blocks) % W);
+            for (long long i = start; i < blocks; i += W) {
+                rows[1].load(p, b + i * 16, e, c0);
+                if (held) rows[0].multiply(acc);
+                rows[0] = rows[1];
+                held = true;
             }
         }
     }
+    if (held) rows[0].multiply(acc);
     O* out = (O*)p.out + (long long)ad * p.rank * p.N;
 #pragma unroll
     for (int q = 0; q < NRB; ++q) {
@@ -175,7 +297,9 @@ proj_factor_kernel(ProjFactor p) {
             for (int j = 0; j < 4; ++j) {
                 const int c = n0 + lh * 16 + u * 4 + j;
                 if (c >= p.N) continue;
-                const float v = acc[q][j][u] + part[0][j][lane][u] + part[1][j][lane][u] + part[2][j][lane][u];
+                float v = acc[q][j][u];
+#pragma unroll
+                for (int w = 0; w < W - 1; ++w) v += part[w][j][lane][u];
                 out[p.by_col ? (long long)c * p.rank + k : (long long)k * p.N + c] = pj_from_f32<ODT>(v);
             }
     }
@@ -208,25 +332,32 @@ template <int DT, int NRB>
 static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool xv = pj_aligned(p.x, p.ldx, E, 16) && p.K % V == 0;
-    const bool fv = p.f_k == 1 && pj_aligned(p.f, p.f_rank, E, 16) && p.K % V == 0;
+    const bool fk = p.f_k == 1 && pj_aligned(p.f, p.f_rank, E, 16) && p.K % V == 0;
+    const bool fr = DT != VDB_F32 && p.f_rank == 1 && p.f_k == p.rank && p.rank % 8 == 0 && (uintptr_t)p.f % 16 == 0;
     const long long blocks = (p.n + 15) / 16;
-    long long share = (p.segments + blocks - 1) / blocks;       // requests per block of rows, if they are of one length
+    // workgroups for the adapters of one block: twice as many as it meets if all requests were of one length, and enough to fill
+    // the chip: one that finds nothing to do costs less than adapters one after the other
+    long long share = 2 * (long long)p.segments / blocks;
+    if (share < 1024 / blocks) share = 1024 / blocks;
+    if (share > p.segments) share = p.segments;
     share = share < 1 ? 1 : share > 16 ? 16 : share;
     const dim3 grid((unsigned)(blocks * share));
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, (int)share);
         return hipGetLastError();
     };
-    if (!xv) return fv ? go(proj_shrink_kernel<DT, NRB, false, true>) : go(proj_shrink_kernel<DT, NRB, false, false>);
-    return fv ? go(proj_shrink_kernel<DT, NRB, true, true>) : go(proj_shrink_kernel<DT, NRB, true, false>);
+    if (!xv || !(fk || fr)) return go(proj_shrink_kernel<DT, NRB, false, PJ_S_ANY>);
+    if constexpr (DT != VDB_F32) if (!fk) return go(proj_shrink_kernel<DT, NRB, true, PJ_S_FR>);
+    return go(proj_shrink_kernel<DT, NRB, true, PJ_S_FK>);
 }
 
 template <int DT, int ODT, int NRB>
 static hipError_t factor_typed(const ProjFactor& p, hipStream_t st) {
-    const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)p.adapters);
+    const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)p.adapters), threads(PJ_FACTOR_WAVES * 64);
     const bool xv = pj_aligned(p.x, p.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && p.N % 4 == 0;
-    return xv ? pj_launch(proj_factor_kernel<DT, ODT, NRB, true>, grid, 0, p, st)
-              : pj_launch(proj_factor_kernel<DT, ODT, NRB, false>, grid, 0, p, st);
+    if (xv) hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, true>), grid, threads, 0, st, p);
+    else hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, false>), grid, threads, 0, st, p);
+    return hipGetLastError();
 }
 
 // blocks of 16 of the rank, rounded up to a power of two

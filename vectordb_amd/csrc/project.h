@@ -26,8 +26,8 @@ struct ProjRows {
     long long n; int N, K;
     int dtype, out_dtype;
     const long long* offsets; int segments;
-    // low-rank term: y_i += sum_q h[i][q] f[adapter][column][q]; null ids: none
-    const int* ids; int adapters;
+    // low-rank term: y_i += sum_q h[i][q] f[row_adapter[i]][column][q]; null: none
+    const int* row_adapter;              // [n], -1: none
     const void* h;                       // [n][proj_parts][proj_rank_pad]
     const float* h_scale;                // fp16: [n], what the parts of a row have to be multiplied with
     const void* f; long long f_adapter, f_col, f_rank;       // strides in elements
@@ -40,6 +40,7 @@ struct ProjShrink {
     const void* f; long long f_adapter, f_rank, f_k;
     const float* scale;
     void* h; float* h_scale;             // parts, see ProjRows; null: not wanted
+    int* row_adapter;                    // [n]: the adapter of each row, -1: none; may be null
     float* h32; int rp32;                // [n][rp32] fp32; null: not wanted
     int rank, dtype;
     const long long* offsets; int segments; const int* ids; int adapters;

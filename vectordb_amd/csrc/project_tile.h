@@ -110,12 +110,18 @@ __device__ __forceinline__ int pj_first_segment(const long long* offsets, int se
     return lo;
 }
 
+// (a shuffle of a lane that is the same for all goes through LDS: 0.1 us for each request)
+__device__ __forceinline__ long long pj_readlane64(long long v, int lane) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)v, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+
 // Requests with an adapter that meet rows [r0, r1): visited one by one by the whole wave, 64 loaded at a time.
 template <typename F>
 __device__ __forceinline__ void pj_each_request(const long long* offsets, const int* ids, int segments, int adapters, long long n,
                                                 long long r0, long long r1, F&& visit) {
     const int lane = threadIdx.x & 63;
-    for (int s0 = pj_first_segment(offsets, segments, r0); s0 < segments; s0 += 64) {
+    for (int s0 = segments <= 64 ? 0 : pj_first_segment(offsets, segments, r0); s0 < segments; s0 += 64) {
         const int s = s0 + lane;
         long long b = n, e = 0;
         int a = -1;
@@ -125,7 +131,7 @@ __device__ __forceinline__ void pj_each_request(const long long* offsets, const 
         while (m) {
             const int src = __builtin_ctzll(m);
             m &= m - 1;
-            visit(__shfl(b, src), __shfl(e, src), __builtin_amdgcn_readlane(a, src));
+            visit(pj_readlane64(b, src), pj_readlane64(e, src), __builtin_amdgcn_readlane(a, src));
         }
         if (last) break;
     }
@@ -353,21 +359,6 @@ struct PJProduct {
 //     so that what one adapter holds never reaches another request's rows;
 //   more: every lane for itself, its row by its four columns, which waits once for all adapters instead of once for each.
 
-// Adapter of each of B times 16 rows (lane l: row + 16 i + l % 16); -1: none.
-template <int B>
-__device__ __forceinline__ void pj_row_adapters(const ProjRows& p, long long row, int (&am)[B]) {
-    const int li = threadIdx.x & 15;
-#pragma unroll
-    for (int i = 0; i < B; ++i) am[i] = -1;
-    pj_each_request(p.offsets, p.ids, p.segments, p.adapters, p.n, row, row + B * 16, [&](long long b, long long e, int a) {
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const long long m = row + i * 16 + li;
-            am[i] = m >= b && m < e ? a : am[i];
-        }
-    });
-}
-
 // How the factor f lies: entry (column, rank) of an adapter at column * f_col + rank * f_rank elements (32 bits hold it).
 //   PJ_F_RANKS   ranks contiguous, 16-byte pieces of them aligned (B of a forward pass)
 //   PJ_F_COLS    columns contiguous, groups of four aligned and whole (A of a backward pass)
@@ -456,14 +447,23 @@ __device__ __forceinline__ void pj_low_rank_lanes(const ProjRows& p, long long m
     }
 }
 
-// B blocks of 16 rows from `row`, C of 16 columns from `colb`.  `waves` > 1: that many waves share the block, and the sum of
+// Adapters of B blocks of 16 rows (lane l: row + 16 i + l % 16); -1: none.
+template <int B> __device__ __forceinline__ void pj_load_adapters(const ProjRows& p, long long row, int (&am)[B]) {
+    const int li = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const long long m = row + i * 16 + li;
+        am[i] = m < p.n ? p.row_adapter[m] : -1;
+    }
+}
+
+// B blocks of 16 rows from `row`, C of 16 columns from `colb`; am: the rows' adapters.  `waves` > 1: that many waves share the block, and the sum of
 // their accumulators is the term.
 template <int DT, int F, int B, int C>
-__device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, int colb, pj_f32x4 (&acc)[B][C], int waves = 1, int wave = 0) {
+__device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, int colb, const int (&am)[B], pj_f32x4 (&acc)[B][C],
+                                            int waves = 1, int wave = 0) {
     constexpr int V = 16 / PJ<DT>::E;
     const int li = threadIdx.x & 15;
-    int am[B];
-    pj_row_adapters<B>(p, row, am);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
         const long long m = row + i * 16 + li, mc = m < p.n ? m : p.n - 1;
@@ -532,8 +532,10 @@ proj_rows_kernel(PJRowsArgs a) {
     PJProduct<DT, false, NK, VEC, R> prod;
     prod.om.init((const T*)p.x, p.ldx, row0, row1);
     prod.on.init((const T*)p.w + (long long)seg * p.w_group, p.ldw, col0, p.N);
+    int am[B] = {};
+    if constexpr (ADAPT) pj_load_adapters<B>(p, row0 + wm * (R / 2), am);        // before the stages' loads, which return in order
     prod.begin(p.K, pj_lds);
-    if constexpr (ADAPT) pj_low_rank<DT, F, B, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), acc);
+    if constexpr (ADAPT) pj_low_rank<DT, F, B, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), am, acc);
     prod.run(pj_lds, wm, wn, acc);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -574,7 +576,11 @@ proj_few_kernel(PJRowsArgs a) {
     const T* x = (const T*)p.x + (m < row1 ? m : row1 - 1) * p.ldx;
     const T* w = (const T*)p.w + (long long)seg * p.w_group + (NK ? (c < p.N ? c : p.N - 1) : (long long)(c < p.N ? c : p.N - 1) * p.ldw);
     pj_f32x4 acc[1][1] = {};
-    if constexpr (ADAPT) pj_low_rank<DT, F, 1, 1>(p, row0, col * 16, acc, 4, wave);
+    if constexpr (ADAPT) {
+        int am[1];
+        pj_load_adapters<1>(p, row0, am);
+        pj_low_rank<DT, F, 1, 1>(p, row0, col * 16, am, acc, 4, wave);
+    }
     for (int k0 = wave * KS; k0 < p.K; k0 += U * 4 * KS) {
         union frag { T t[V]; pj_u32x4 v; } xa[U], wa[U];
 #pragma unroll
@@ -656,7 +662,7 @@ static inline bool pj_small_tiles(long long tiles128) { return tiles128 < 256; }
 
 // The low-rank factor can be read in vectors: forward its ranks are contiguous, backward its columns.
 template <int DT, int V> static bool pj_factor_vec(const ProjRows& p) {
-    if (!p.ids) return false;
+    if (!p.row_adapter) return false;
     return p.f_rank == 1 ? p.rank % V == 0 && (uintptr_t)p.f % 16 == 0
                          : p.N % 4 == 0 && (uintptr_t)p.f % (4 * PJ<DT>::E) == 0;
 }
@@ -668,18 +674,18 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     a.col_tiles = (p.N + R - 1) / R;
     constexpr int E = PJ<DT>::E, V = 16 / E;
     a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 4 * PJ<ODT>::E);
-    const long long row_tiles = p.ids ? (p.n + R - 1) / R : p.n / R + p.segments;
+    const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + p.segments;
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const size_t lds = PJRing<R>::BYTES;
     const bool fv = pj_factor_vec<DT, V>(p);
 #define PJ_ROWS(NK, VEC)                                                                              \
-    (!p.ids ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY, R>, grid, lds, a, st)     \
+    (!p.row_adapter ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY, R>, grid, lds, a, st)     \
      : fv   ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st) \
             : pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, PJ_F_ANY, R>, grid, lds, a, st))
     if constexpr (R == 128) {
         // (a factor that cannot be read in vectors would spill here)
 #define PJ_BIG(NK)                                                                                                        \
-    (p.ids ? pj_launch(proj_rows_kernel<DT, ODT, NK, true, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st)       \
+    (p.row_adapter ? pj_launch(proj_rows_kernel<DT, ODT, NK, true, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st)       \
            : pj_launch(proj_rows_kernel<DT, ODT, NK, true, false, PJ_F_ANY, R>, grid, lds, a, st))
         return p.w_by_k ? PJ_BIG(true) : PJ_BIG(false);
 #undef PJ_BIG
@@ -697,11 +703,11 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
     a.col_tiles = (p.N + 15) / 16;
     constexpr int V = 16 / PJ<DT>::E;
     a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 4 * PJ<ODT>::E);
-    const long long row_tiles = p.ids ? (p.n + 15) / 16 : p.n / 16 + p.segments;
+    const long long row_tiles = p.row_adapter ? (p.n + 15) / 16 : p.n / 16 + p.segments;
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const bool fv = pj_factor_vec<DT, V>(p);
 #define PJ_FEW(NK, VEC)                                                                          \
-    (!p.ids ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY>, grid, 0, a, st)      \
+    (!p.row_adapter ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY>, grid, 0, a, st)      \
      : fv   ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, true, NK ? PJ_F_COLS : PJ_F_RANKS>, grid, 0, a, st) \
             : pj_launch(proj_few_kernel<DT, ODT, NK, VEC, true, PJ_F_ANY>, grid, 0, a, st))
     if (p.w_by_k) return vec ? PJ_FEW(true, true) : PJ_FEW(true, false);
@@ -718,10 +724,10 @@ static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool vec = pj_aligned(p.x, p.ldx, E, 16) && pj_aligned(p.w, p.ldw, E, 16) && p.w_group % V == 0 &&
                      p.K % V == 0 && (!p.w_by_k || p.N % V == 0);
-    const long long tiles = ((p.n + 127) / 128 + (p.ids ? 0 : p.segments / 2)) * ((p.N + 127) / 128);
+    const long long tiles = ((p.n + 127) / 128 + (p.row_adapter ? 0 : p.segments / 2)) * ((p.N + 127) / 128);
     const long long tiles64 = ((p.n + 63) / 64) * ((p.N + 63) / 64);
     if (tiles64 <= PJ_FEW_TILES) return pj_few<DT, ODT>(p, vec, st);
-    const bool big = vec && !pj_small_tiles(tiles) && (!p.ids || pj_factor_vec<DT, V>(p));
+    const bool big = vec && !pj_small_tiles(tiles) && (!p.row_adapter || pj_factor_vec<DT, V>(p));
     return big ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
 }
 
