@@ -200,6 +200,38 @@ def test_grouped(engine, case, dtype, out):
     Case(n, din, dout, off, dtype, out).check(engine)
 
 
+# rows enough for the gradient of the matrices to be summed in chunks, and for every shape of tile
+LARGE = [
+    (2000, 136, 72, [0, 1500, 1500, 1501, 2000]),
+    (3001, 67, 45, [5, 1000, 2990]),
+    (1300, 384, 384, [0, 400, 400, 1300]),
+    (9000, 256, 520, [0, 3, 5000, 9000]),
+    (40000, 136, 768, [0, 20000, 20000, 39990]),
+    (16000, 768, 640, [100, 7000, 7001, 16000]),
+    (70000, 128, 272, [0, 12345, 70000]),
+]
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: "%dx%dx%d_%dg" % (c[0], c[1], c[2], len(c[3]) - 1))
+def test_grouped_large(engine, case, dtype, out):
+    n, din, dout, off = case
+    Case(n, din, dout, off, dtype, out).check(engine)
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,rank", [(3000, 128, 200, 16), (20000, 256, 768, 24), (52000, 128, 264, 8), (9000, 520, 256, 100)])
+def test_adapted_large(engine, n, din, dout, rank, dtype, out):
+    """Requests of very different length: one row, a few, thousands; many adapters within 16 rows and one over many tiles."""
+    lens = [1] * 40 + [3] * 20 + [n // 3, 0, 17, 1, 100] + [n // 5]
+    off = [0]
+    for v in lens:
+        off.append(off[-1] + v)
+    off.append(n - 9)
+    ids = [(5 * i) % 12 - 1 for i in range(len(off) - 1)]
+    Case(n, din, dout, off, dtype, out, 11, rank, ids).check(engine)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shift,pad", [(1, 0), (0, 3), (4, 8), (8, 16), (3, 5)])
 def test_grouped_strides_and_alignment(engine, dtype, shift, pad):
@@ -293,10 +325,12 @@ def test_infinite_row_without_an_adapter_gives_what_the_formula_gives(engine):
 @pytest.mark.parametrize("offsets", [[5, 3, 60, 20, 70], [-4, 10, 90, 1000, 1 << 40], [-9, -9, -1, -1, 0], [99, 99, 99, 99, 99],
                                      [1 << 62, -(1 << 62), 1 << 62, 0, 70], [0, 70, 0, 70, 0]])
 @pytest.mark.parametrize("adapted", [False, True])
-def test_offsets_that_are_wrong_reach_nothing_outside(engine, offsets, adapted):
+@pytest.mark.parametrize("times", [1, 100, 700])
+def test_offsets_that_are_wrong_reach_nothing_outside(engine, offsets, adapted, times):
     """Values of rows in such segments are undefined; the bytes around every output stay, and the call returns."""
-    n = 70
-    c = Case(n, 64, 48, offsets, "bf16", "f32", *((3, 8, [0, 1, 2, 5]) if adapted else ()))
+    n, offsets = 70 * times, [o * times if abs(o) < 1 << 41 else o for o in offsets]
+    ids = [i % 6 for i in range(len(offsets) - 1)]
+    c = Case(n, 128, 48 if times < 700 else 520, offsets, "bf16", "f32", *((3, 8, ids) if adapted else ()))
     y = c.forward(engine)
     torch.cuda.synchronize()
     c.frame(c.buf, y)

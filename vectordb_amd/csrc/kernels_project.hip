@@ -42,12 +42,8 @@ __device__ __forceinline__ void pj_shrink_load_x(const ProjShrink& p, const type
 #pragma unroll
     for (int u = 0; u < XS; ++u) {
         const int k = k0 + u * stride + lh * V;
-        union { T t[V]; pj_u32x4 v; } f;
-        if constexpr (XV) f.v = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
-        else
-#pragma unroll
-            for (int j = 0; j < V; ++j) f.t[j] = k + j < p.K ? x[k + j] : (T)0;
-        xa[u] = f.v;
+        if constexpr (XV) xa[u] = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
+        else xa[u] = pj_piece<T>(x + k, p.K - k);
     }
 }
 
@@ -160,6 +156,11 @@ __device__ __forceinline__ void pj_row_adapters(const ProjShrink& p, long long r
     });
 }
 
+// LDS of pj_shrink_block: the waves' sums, and each wave's lines
+template <int DT, int NRB, int F> constexpr int pj_shrink_block_lds() {
+    return 3 * NRB * 1024 + 4 * pj_shrink_lds<DT, NRB, F, (NRB <= 2 ? 4 : 2)>();
+}
+
 // h = s x f^T for 16 rows: the four waves take every fourth step of the contracted axis and add up through LDS in wave
 // order.  Each adapter that the 16 rows meet is multiplied on its own and keeps its own rows; `share` workgroups divide
 // the adapters of a block of rows among them.  The rows are loaded before the adapters are known.
@@ -167,15 +168,13 @@ __device__ __forceinline__ void pj_row_adapters(const ProjShrink& p, long long r
 // to a workgroup, which reads the factor a quarter as often, were both slower (56 and 45 against 47 us for 32 768 x 1024 rows of
 // rank 64, 24 and 26 against 18 us for 16 384 x 768 of rank 16).
 template <int DT, int NRB, bool XV, int F>
-__global__ void __launch_bounds__(256)
-proj_shrink_kernel(ProjShrink p, int share) {
+__device__ __forceinline__ void pj_shrink_block(const ProjShrink& p, long long r0, int mine, int share, char* smem) {
     typedef typename PJ<DT>::T T;
     constexpr int KS = 64 / PJ<DT>::E, XS = 8, U = NRB <= 2 ? 4 : 2;
-    __shared__ pj_f32x4 part[3][NRB][64];
-    __shared__ __attribute__((aligned(16))) char lds[4][pj_shrink_lds<DT, NRB, F, U>()];
     const int lane = threadIdx.x & 63, li = lane & 15, wave = threadIdx.x >> 6;
-    const long long r0 = (long long)(blockIdx.x / share) * 16, m = r0 + li;
-    const int mine = blockIdx.x % share;
+    pj_f32x4 (*const part)[NRB][64] = (pj_f32x4 (*)[NRB][64])smem;
+    char* const lds = smem + 3 * NRB * 1024 + wave * pj_shrink_lds<DT, NRB, F, U>();
+    const long long m = r0 + li;
     const T* x = (const T*)p.x + (m < p.n ? m : p.n - 1) * p.ldx;
     pj_u32x4 xa[XS];
     pj_shrink_load_x<DT, XS, XV>(p, x, wave * KS, 4 * KS, xa);
@@ -193,7 +192,7 @@ proj_shrink_kernel(ProjShrink p, int share) {
             if (p.K > XS * 4 * KS) pj_shrink_load_x<DT, XS, XV>(p, x, kc, 4 * KS, xa);
 #pragma unroll
             for (int u = 0; u < XS; u += U)
-                if (kc + u * 4 * KS < p.K) pj_shrink_steps<DT, NRB, F, U>(p, xa + u, f, kc + u * 4 * KS, 4 * KS, lds[wave], acc);
+                if (kc + u * 4 * KS < p.K) pj_shrink_steps<DT, NRB, F, U>(p, xa + u, f, kc + u * 4 * KS, 4 * KS, lds, acc);
         }
         __syncthreads();
         if (wave)
@@ -208,6 +207,94 @@ proj_shrink_kernel(ProjShrink p, int share) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][j] += part[w][i][lane][j];
         pj_shrink_store<DT, NRB>(p, m, am[0] == ad, ad, acc);
+    }
+}
+
+template <int DT, int NRB, bool XV, int F>
+__global__ void __launch_bounds__(256)
+proj_shrink_kernel(ProjShrink p, int share) {
+    __shared__ __attribute__((aligned(16))) char smem[pj_shrink_block_lds<DT, NRB, F>()];
+    pj_shrink_block<DT, NRB, XV, F>(p, (long long)(blockIdx.x / share) * 16, blockIdx.x % share, share, smem);
+}
+
+// Many rows of long requests: 64 rows by all ranks through LDS, a ring of four stages of 128 bytes of k as in PJProduct, each
+// wave 16 rows.  For every adapter of the 64 rows (up to four) the whole product; 64 rows of more adapters are left to the
+// workgroups behind the first `tiles`, which take 16 rows each as above and have nothing to do otherwise.
+// (32 768 x 1024 rows, rank 64: 47 us by 16 rows, which read the factor four times as often.)
+template <int DT, int NRB, int F>
+__global__ void __launch_bounds__(256)
+proj_shrink_tile_kernel(ProjShrink p, int tiles) {
+    extern __shared__ __attribute__((aligned(16))) char pj_lds[];
+    typedef typename PJ<DT>::T T;
+    constexpr bool FB = F == PJ_S_FR;
+    constexpr int RN = NRB <= 4 ? 64 : 128, KT = 128 / PJ<DT>::E, S = 4, STAGE = pj_tile_bytes(64) + pj_tile_bytes(RN), L = 2 + RN / 32;
+    const int lane = threadIdx.x & 63, li = lane & 15, wave = threadIdx.x >> 6;
+    const bool own = (int)blockIdx.x < tiles;
+    const long long block = (long long)blockIdx.x - tiles;                   // of 16 rows
+    const long long r0 = own ? (long long)blockIdx.x * 64 : block / 4 * 64;
+    int am[4];
+    pj_row_adapters<4>(p, r0, am);
+    int ads[4], count = 0;                                                  // the adapters in the order of their first rows
+    unsigned left[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { left[i] = (unsigned)__ballot(am[i] >= 0) & 0xffffu; ads[i] = -1; }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        int ad = -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (ad < 0 && left[i]) ad = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left[i]));
+        if (ad < 0) continue;
+        ads[c] = ad;
+        ++count;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) left[i] &= ~(unsigned)__ballot(am[i] == ad);
+    }
+    const bool many = (left[0] | left[1] | left[2] | left[3]) != 0;
+    if (own == many) return;                                                // (for the other kind of workgroup)
+    if (many) {
+        static_assert(pj_shrink_block_lds<DT, NRB, F>() <= S * STAGE, "the ring's memory");
+        pj_shrink_block<DT, NRB, true, F>(p, block * 16, 0, 1, pj_lds);
+        return;
+    }
+    const int mine = wave == 0 ? am[0] : wave == 1 ? am[1] : wave == 2 ? am[2] : am[3];
+    const long long m = r0 + wave * 16 + li;
+    if (p.row_adapter && lane < 16 && m < p.n) p.row_adapter[m] = mine;
+    for (int c = 0; c < count; ++c) {
+        const int ad = c == 0 ? ads[0] : c == 1 ? ads[1] : c == 2 ? ads[2] : ads[3];
+        const T* f = (const T*)p.f + (long long)ad * p.f_adapter;
+        PJOperand<DT, false, 64> ox;
+        PJOperand<DT, FB, RN> of;
+        ox.init((const T*)p.x, p.ldx, r0, p.n);
+        of.init(f, FB ? p.f_k : p.f_rank, 0, p.rank);
+        long long k = p.K;
+        auto next = [&](int stage) {
+            const int l = k < KT ? (k > 0 ? (int)k : 0) : KT;
+            ox.stage(pj_lds + stage * STAGE, l);
+            of.stage(pj_lds + stage * STAGE + pj_tile_bytes(64), l);
+            k -= KT;
+        };
+        __syncthreads();                                                    // the last adapter's stages have been read
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) next(i);
+        pj_f32x4 acc[NRB] = {};
+        const int steps = (p.K + KT - 1) / KT;
+        int cur = 0;
+        for (int t = 0; t < steps; ++t) {
+            pj_wait_and_meet<(S - 2) * L>();
+            next(cur == 0 ? S - 1 : cur - 1);
+            const char* lx = pj_lds + cur * STAGE;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                pj_u32x4 fx[1], ff[NRB];
+                pj_fragments<DT, false, 64, 1>(lx, wave * 16, kk, fx);
+                pj_fragments<DT, FB, RN, NRB>(lx + pj_tile_bytes(64), 0, kk, ff);
+#pragma unroll
+                for (int i = 0; i < NRB; ++i) acc[i] = pj_mfma<DT>(ff[i], fx[0], acc[i]);
+            }
+            cur = cur + 1 == S ? 0 : cur + 1;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        pj_shrink_store<DT, NRB>(p, m, mine == ad, ad, acc);
     }
 }
 
@@ -305,6 +392,49 @@ proj_factor_kernel(ProjFactor p) {
     }
 }
 
+// dw of the segments that were split, and zeros for those without rows: the chunks' partial sums in their order.
+template <int ODT>
+__global__ void __launch_bounds__(256)
+proj_weights_sum_kernel(ProjWeights p) {
+    typedef typename PJ<ODT>::T O;
+    const int seg = blockIdx.y, lane = threadIdx.x & 63;
+    const long long size = (long long)p.M * p.N;
+    long long first = 0;                     // number of the segment's first chunk
+    for (int s0 = 0; s0 < seg; s0 += 64) {
+        long long c = 0;
+        if (s0 + lane < seg) {
+            const long long b = pj_clamp(p.offsets[s0 + lane], p.n), e = pj_clamp(p.offsets[s0 + lane + 1], p.n);
+            c = e > b ? (e - b + p.chunk - 1) / p.chunk : 0;
+        }
+        for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o);
+        first += c;
+    }
+    const long long b = pj_clamp(p.offsets[seg], p.n), e = pj_clamp(p.offsets[seg + 1], p.n);
+    long long chunks = e > b ? (e - b + p.chunk - 1) / p.chunk : 0;
+    if (chunks == 1) return;
+    const long long room = p.n / p.chunk + p.segments - first;       // offsets that decrease could name more chunks than there are
+    if (chunks > room) chunks = room < 0 ? 0 : room;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (long long)gridDim.x * 1024) {
+        const float* in = p.partial + first * size + i;
+        pj_f32x4 v = {};
+        if (size % 4 == 0) {
+#pragma unroll 4
+            for (long long c = 0; c < chunks; ++c) {
+                const pj_f32x4 t = *(const pj_f32x4*)(in + c * size);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += t[j];
+            }
+        } else {
+            for (long long c = 0; c < chunks; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (i + j < size) v[j] += in[c * size + j];
+        }
+        O* out = (O*)p.dw + seg * size + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (i + j < size) out[j] = pj_from_f32<ODT>(v[j]);
+    }
+}
+
 __global__ void __launch_bounds__(256)
 proj_zero_outside_kernel(float* q, long long dim, long long n, const long long* offsets, int segments) {
     const long long b = segments > 0 ? pj_clamp(offsets[0], n) : 0, e = segments > 0 ? pj_clamp(offsets[segments], n) : 0;
@@ -328,17 +458,51 @@ hipError_t launch_proj_rows(const ProjRows& p, hipStream_t st) {
 
 hipError_t launch_proj_weights(const ProjWeights& p, hipStream_t st) { PJ_BY_TYPE(launch_proj_weights); }
 
+hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st) {
+    const long long size = (long long)p.M * p.N;
+    long long blocks = (size + 1023) / 1024;
+    if (blocks > 1024) blocks = 1024;
+    const dim3 grid((unsigned)blocks, (unsigned)p.segments);
+    if (p.out_dtype == VDB_F32) return pj_launch(proj_weights_sum_kernel<VDB_F32>, grid, 0, p, st);
+    if (p.out_dtype == VDB_BF16) return pj_launch(proj_weights_sum_kernel<VDB_BF16>, grid, 0, p, st);
+    return pj_launch(proj_weights_sum_kernel<VDB_F16>, grid, 0, p, st);
+}
+
+// Rows, and average length of a request, from which the shrink works by 64 rows.
+#ifndef PJ_SHRINK_TILE_ROWS
+#define PJ_SHRINK_TILE_ROWS 8192
+#endif
+#ifndef PJ_SHRINK_TILE_LEN
+#define PJ_SHRINK_TILE_LEN 128
+#endif
 template <int DT, int NRB>
 static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool xv = pj_aligned(p.x, p.ldx, E, 16) && p.K % V == 0;
     const bool fk = p.f_k == 1 && pj_aligned(p.f, p.f_rank, E, 16) && p.K % V == 0;
+    const bool ftile = p.f_rank == 1 && p.f_k == p.rank && p.rank % V == 0 && (uintptr_t)p.f % 16 == 0;
     const bool fr = DT != VDB_F32 && p.f_rank == 1 && p.f_k == p.rank && p.rank % 8 == 0 && (uintptr_t)p.f % 16 == 0;
     const long long blocks = (p.n + 15) / 16;
-    // workgroups for the adapters of one block: twice as many as it meets if all requests were of one length, and enough to fill
-    // the chip: one that finds nothing to do costs less than adapters one after the other
-    long long share = 2 * (long long)p.segments / blocks;
-    if (share < 1024 / blocks) share = 1024 / blocks;
+    if (p.n >= PJ_SHRINK_TILE_ROWS && p.n / p.segments >= PJ_SHRINK_TILE_LEN && xv && (fk || ftile)) {
+        const int tiles = (int)((p.n + 63) / 64);
+        const dim3 grid((unsigned)(tiles + blocks));
+        const size_t lds = 4 * (pj_tile_bytes(64) + pj_tile_bytes(NRB <= 4 ? 64 : 128));
+        auto go = [&](auto kernel) {
+            if (lds > 65536) {
+                const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+                if (e != hipSuccess) return e;
+            }
+            hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, p, tiles);
+            return hipGetLastError();
+        };
+        if (fk) return go(proj_shrink_tile_kernel<DT, NRB, PJ_S_FK>);
+        return go(proj_shrink_tile_kernel<DT, NRB, PJ_S_FR>);
+    }
+    // workgroups for the adapters of one block: as many as it meets if all requests were of one length, and a workgroup to a CU.
+    // More are dispatched in vain (1024 rows of 128 requests: 12.4 us with 256 workgroups in all, 15.1 with 1024), fewer leave
+    // adapters one after the other (15.8 us with 128).
+    long long share = (long long)p.segments / blocks;
+    if (share < 256 / blocks) share = 256 / blocks;
     if (share > p.segments) share = p.segments;
     share = share < 1 ? 1 : share > 16 ? 16 : share;
     const dim3 grid((unsigned)(blocks * share));

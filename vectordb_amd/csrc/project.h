@@ -9,6 +9,9 @@
 namespace vdb {
 
 constexpr int PROJ_MAX_RANK = 128;
+#ifndef PJ_SPLIT_WGS
+#define PJ_SPLIT_WGS 768
+#endif
 // A low-rank intermediate h [n, rank], fp32, is handed to the kernel that multiplies it as parts of the rows' type that add up
 // to it: rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks for 16-bit types, 16 for fp32).
 __host__ __device__ constexpr int proj_parts(int dtype) { return dtype == VDB_F32 ? 1 : dtype == VDB_BF16 ? 3 : 2; }
@@ -53,7 +56,24 @@ struct ProjWeights {
     void* dw; int M, N;                  // [segments][M][N]
     long long n; int dtype, out_dtype;
     const long long* offsets; int segments;
+    int tile;                            // 128 or 64, see proj_weights_plan
+    int chunk;                           // rows per workgroup where segments are split, 0: they are not
+    float* partial;                      // chunk > 0: [n / chunk + segments][M][N]
 };
+
+// How the gradient of the matrices is divided: 128 x 128 output tiles where they fill half the chip by themselves, or would with
+// segments of 2048 rows split; 64 x 64 ones otherwise; and chunks of rows that give every CU two workgroups.
+inline void proj_weights_plan(long long n, int segments, int M, int N, int& tile, int& chunk) {
+    const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128), t64 = (long long)((M + 63) / 64) * ((N + 63) / 64);
+    tile = segments * t128 >= 256 || n / 2048 * t128 >= 256 ? 128 : 64;
+    const long long tiles = tile == 128 ? t128 : t64;
+    chunk = 0;
+    if (segments * tiles >= PJ_SPLIT_WGS) return;
+    long long c = (n * tiles + PJ_SPLIT_WGS - 1) / PJ_SPLIT_WGS;
+    c = (c + 63) / 64 * 64;
+    if (c < 128) c = 128;
+    if (c < n) chunk = (int)c;
+}
 
 // out[a][q][c] (or, by_col, out[a][c][q]) = sum over the rows i of adapter a of h[i][q] x[i][c]
 struct ProjFactor {
@@ -73,6 +93,7 @@ hipError_t launch_proj_weights_bf16(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_weights_f16(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st);
 hipError_t launch_proj_weights(const ProjWeights& p, hipStream_t st);
+hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st);      // the second step where segments are split
 hipError_t launch_proj_factor(const ProjFactor& p, hipStream_t st);
 // rows [n, dim] of q outside every segment become zero
 hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st);

@@ -40,6 +40,22 @@ template <int DT> __device__ __forceinline__ typename PJ<DT>::T pj_from_f32(floa
     else return __builtin_bit_cast(unsigned short, (_Float16)v);
 }
 
+// Vectors at any address that is aligned to an element of 16 bits.
+typedef pj_u32x4 pj_u32x4_any __attribute__((aligned(2)));
+typedef pj_f32x4 pj_f32x4_any __attribute__((aligned(4)));
+typedef pj_s16x4 pj_s16x4_any __attribute__((aligned(2)));
+
+// The 16 bytes at p of which `left` elements lie in the operand (none: 0 or less), the others zero.
+template <typename T> __device__ __forceinline__ pj_u32x4 pj_piece(const T* p, int left) {
+    constexpr int V = 16 / sizeof(T);
+    union { T t[V]; pj_u32x4 v; } r;
+    if (left >= V) r.v = *(const pj_u32x4_any*)p;
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) r.t[j] = j < left ? p[j] : (T)0;
+    return r.v;
+}
+
 // ------------------------------------------------------------------------------------------- segments
 __device__ __forceinline__ long long pj_clamp(long long v, long long n) { return v < 0 ? 0 : v > n ? n : v; }
 
@@ -48,7 +64,7 @@ __device__ __forceinline__ long long pj_clamp(long long v, long long n) { return
 // (workgroup b runs on XCD b % 8), so that the column tiles that share rows share an L2.
 // Every wave does this by itself, 64 segments at a time.  Returns false for workgroups past the last tile.
 __device__ __forceinline__ bool pj_find_tile(const long long* offsets, int segments, long long n, int tm, int col_tiles,
-                                             unsigned bid, int& seg, long long& row0, long long& row1, int& col) {
+                                             unsigned bid, int& seg, long long& row0, long long& row1, int& col, long long& number) {
     const int lane = threadIdx.x & 63;
     long long total = 0;
     for (int s0 = 0; s0 < segments; s0 += 64) {
@@ -68,6 +84,7 @@ __device__ __forceinline__ bool pj_find_tile(const long long* offsets, int segme
     if (id >= all) return false;
     col = (int)(id % col_tiles);
     const long long want = id / col_tiles;
+    number = want;
     long long before = 0;
     for (int s0 = 0; s0 < segments; s0 += 64) {
         const int s = s0 + lane;
@@ -90,6 +107,12 @@ __device__ __forceinline__ bool pj_find_tile(const long long* offsets, int segme
         before += __shfl(inc, 63);
     }
     return false;
+}
+
+__device__ __forceinline__ bool pj_find_tile(const long long* offsets, int segments, long long n, int tm, int col_tiles,
+                                             unsigned bid, int& seg, long long& row0, long long& row1, int& col) {
+    long long number;
+    return pj_find_tile(offsets, segments, n, tm, col_tiles, bid, seg, row0, row1, col, number);
 }
 
 // First segment whose end lies behind `row` (offsets do not decrease); `segments` if there is none.  Called by whole
@@ -182,26 +205,27 @@ template <int DT, bool BYK, int R> struct PJOperand {
         }
     }
     // the next KT elements of the contracted axis, of which `kleft` lie in the operand: one load per piece whatever kleft is
-    template <bool VEC> __device__ __forceinline__ void stage(char* lds, int kleft) {
+    __device__ __forceinline__ void stage(char* lds, int kleft) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             char* const wave_dst = lds + (i * PJ_THREADS + ((int)threadIdx.x & ~63)) * 16;
-            if constexpr (VEC) {
-                const T* s = rem[i] && kpos[i] < kleft ? src[i] : (const T*)pj_zero16;
-                __builtin_amdgcn_global_load_lds((const PJ_GLOBAL void*)s, (PJ_LOCAL void*)wave_dst, 16, 0, 0);
-            } else {
-                T v[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const bool ok = BYK ? (j < rem[i] && kpos[i] < kleft) : (rem[i] && kpos[i] + j < kleft);
-                    v[j] = ok ? src[i][j] : (T)0;
-                }
-                T* d = (T*)(wave_dst + ((int)threadIdx.x & 63) * 16);
-#pragma unroll
-                for (int j = 0; j < V; ++j) d[j] = v[j];
-            }
+            const T* s = rem[i] && kpos[i] < kleft ? src[i] : (const T*)pj_zero16;
+            __builtin_amdgcn_global_load_lds((const PJ_GLOBAL void*)s, (PJ_LOCAL void*)wave_dst, 16, 0, 0);
             src[i] += step[i];
         }
+    }
+    // the same for operands of any alignment and size, through registers
+    __device__ __forceinline__ void load(pj_u32x4 (&r)[P], int kleft) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int left = BYK ? (kpos[i] < kleft ? rem[i] : 0) : (rem[i] ? kleft - kpos[i] : 0);
+            r[i] = pj_piece<T>(src[i], left);
+            src[i] += step[i];
+        }
+    }
+    __device__ __forceinline__ void put(char* lds, const pj_u32x4 (&r)[P]) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) *(pj_u32x4*)(lds + (i * PJ_THREADS + (int)threadIdx.x) * 16) = r[i];
     }
 };
 
@@ -225,7 +249,14 @@ __device__ __forceinline__ void pj_fragments(const char* lds, int row, int kk, p
             for (int j = 0; j < 4; ++j)
                 f[i][j] = *(const unsigned*)(lds + (kk * 16 + lh * 4 + j) * LINE + (c << 4) + (li & 3) * 4);
         }
+    } else if constexpr (B == 8) {
+        pj_u32x4 lo[4], hi[4];
+        pj_fragments<DT, BYK, R, 4>(lds, row, kk, lo);
+        pj_fragments<DT, BYK, R, 4>(lds, row + 64, kk, hi);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
     } else {
+        static_assert(B == 2 || B == 4, "fragments of one asm block");
         // ds_read_b64_tr_b16: sixteen lanes read a block of 4 k x 16 rows, lane i the 8 bytes number i % 4 of line i / 4, and get
         // column i of the block; lines k and k + 4 have the same swizzle.  The reads and their wait are one asm block: through
         // the builtin the compiler waits for every load into LDS in flight first.
@@ -272,15 +303,15 @@ template <int DT> __device__ __forceinline__ pj_f32x4 pj_mfma(const pj_u32x4& a,
 }
 
 // Stores the four consecutive columns that a lane holds of one row; `left` of them lie in the output.
-template <int DT> __device__ __forceinline__ void pj_store4(void* out, long long at, const pj_f32x4& v, long long left, bool vec) {
+template <int DT> __device__ __forceinline__ void pj_store4(void* out, long long at, const pj_f32x4& v, long long left) {
     typedef typename PJ<DT>::T T;
     T* p = (T*)out + at;
     T t[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) t[j] = pj_from_f32<DT>(v[j]);
-    if (vec && left >= 4) {
-        if constexpr (DT == VDB_F32) *(pj_f32x4*)p = v;
-        else { pj_s16x4 s = {(short)t[0], (short)t[1], (short)t[2], (short)t[3]}; *(pj_s16x4*)p = s; }
+    if (left >= 4) {
+        if constexpr (DT == VDB_F32) *(pj_f32x4_any*)p = v;
+        else { pj_s16x4 s = {(short)t[0], (short)t[1], (short)t[2], (short)t[3]}; *(pj_s16x4_any*)p = s; }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (j < left) p[j] = t[j];
@@ -312,42 +343,74 @@ struct PJProduct {
     long long left;              // of k, not yet staged
     int tiles;
 
-    __device__ __forceinline__ void next(char* lds, int stage) {
+    // VEC: loads straight into LDS.  Otherwise through D sets of registers, loaded D steps ahead and put into the other half of
+    // the ring while the current step is multiplied.
+    static constexpr int D = 3;
+    pj_u32x4 rm[VEC ? 1 : D][VEC ? 1 : PJOperand<DT, MK, R>::P], rn[VEC ? 1 : D][VEC ? 1 : PJOperand<DT, NK, R>::P];
+
+    __device__ __forceinline__ int take() {
         const int l = left < KT ? (left > 0 ? (int)left : 0) : KT;
-        om.template stage<VEC>(lds + stage * 2 * TB, l);
-        on.template stage<VEC>(lds + stage * 2 * TB + TB, l);
         left -= KT;
+        return l;
+    }
+    __device__ __forceinline__ void next(char* lds, int stage) {
+        const int l = take();
+        om.stage(lds + stage * 2 * TB, l);
+        on.stage(lds + stage * 2 * TB + TB, l);
     }
     __device__ __forceinline__ void begin(long long K, char* lds) {
         left = K;
         tiles = (int)((K + KT - 1) / KT);
-        if (tiles > 0)
+        if (tiles <= 0) return;
+        if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < S - 1; ++i) next(lds, i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < D; ++i) { const int l = take(); om.load(rm[i], l); on.load(rn[i], l); }
+        }
+    }
+    __device__ __forceinline__ void multiply(const char* lm, int wm, int wn, pj_f32x4 (&acc)[B][B]) {
+        const char* ln = lm + TB;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            pj_u32x4 fm[B], fn[B];
+            pj_fragments<DT, MK, R, B>(lm, wm * (R / 2), kk, fm);
+            pj_fragments<DT, NK, R, B>(ln, wn * (R / 2), kk, fn);
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+#pragma unroll
+                for (int j = 0; j < B; ++j) acc[i][j] = pj_mfma<DT>(fn[j], fm[i], acc[i][j]);
+        }
     }
     // acc += om on^T; the wave's block is rows wm * R/2.., columns wn * R/2..
     __device__ __forceinline__ void run(char* lds, int wm, int wn, pj_f32x4 (&acc)[B][B]) {
-        constexpr int L = 2 * PJOperand<DT, MK, R>::P;          // loads per stage and thread
-        int cur = 0;
-        for (int t = 0; t < tiles; ++t) {
-            pj_wait_and_meet<VEC ? (S - 2) * L : 0>();
-            next(lds, cur == 0 ? S - 1 : cur - 1);
-            const char* lm = lds + cur * 2 * TB;
-            const char* ln = lm + TB;
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                pj_u32x4 fm[B], fn[B];
-                pj_fragments<DT, MK, R, B>(lm, wm * (R / 2), kk, fm);
-                pj_fragments<DT, NK, R, B>(ln, wn * (R / 2), kk, fn);
-#pragma unroll
-                for (int i = 0; i < B; ++i)
-#pragma unroll
-                    for (int j = 0; j < B; ++j) acc[i][j] = pj_mfma<DT>(fn[j], fm[i], acc[i][j]);
+        if constexpr (VEC) {
+            constexpr int L = 2 * PJOperand<DT, MK, R>::P;          // loads per stage and thread
+            int cur = 0;
+            for (int t = 0; t < tiles; ++t) {
+                pj_wait_and_meet<(S - 2) * L>();
+                next(lds, cur == 0 ? S - 1 : cur - 1);
+                multiply(lds + cur * 2 * TB, wm, wn, acc);
+                cur = cur + 1 == S ? 0 : cur + 1;
             }
-            cur = cur + 1 == S ? 0 : cur + 1;
+            // nothing may still be on its way into LDS when the workgroup's memory goes to another one
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+            for (int t = 0; t < tiles; t += D)
+#pragma unroll
+                for (int d = 0; d < D; ++d) {
+                    if (t + d >= tiles) break;
+                    char* const buf = lds + ((t + d) & 1) * 2 * TB;
+                    om.put(buf, rm[d]);
+                    on.put(buf + TB, rn[d]);
+                    const int l = take();
+                    om.load(rm[d], l);
+                    on.load(rn[d], l);
+                    __syncthreads();                                // (the other half was read a step ago, before the last meeting)
+                    multiply(buf, wm, wn, acc);
+                }
         }
-        // nothing may still be on its way into LDS when the workgroup's memory goes to another one
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 };
 
@@ -375,7 +438,7 @@ __device__ __forceinline__ void pj_low_rank_block(const ProjRows& p, long long m
     const unsigned fr = (unsigned)p.f_rank, fcol = (unsigned)p.f_col;
     const T* f = (const T*)p.f + (long long)a * p.f_adapter;
     const T* h = (const T*)p.h + mc * (NP * rp);
-#pragma unroll 1
+#pragma unroll F == PJ_F_RANKS ? 2 : 1
     for (int q = 0; q < p.rank; q += QS) {
         pj_u32x4 hv[NP];
 #pragma unroll
@@ -396,6 +459,50 @@ __device__ __forceinline__ void pj_low_rank_block(const ProjRows& p, long long m
     }
 }
 
+// All B blocks of 16 rows by one adapter.
+template <int DT, int F, int B, int C>
+__device__ __forceinline__ void pj_low_rank_all(const ProjRows& p, long long row, int colb, int a, pj_f32x4 (&acc)[B][C]) {
+    typedef typename PJ<DT>::T T;
+    constexpr int V = 16 / PJ<DT>::E, QS = 4 * V, NP = proj_parts(DT);
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    const int rp = proj_rank_pad(p.rank, DT);
+    const unsigned fr = (unsigned)p.f_rank, fcol = (unsigned)p.f_col;
+    const T* f = (const T*)p.f + (long long)a * p.f_adapter;
+    const T* h = (const T*)p.h + (row + li) * (NP * rp);
+#pragma unroll 1
+    for (int q = 0; q < p.rank; q += QS) {
+        const int r = q + lh * V;
+        pj_u32x4 hv[B][NP];
+        union { T t[V]; pj_u32x4 v; } fv[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int col = colb + j * 16 + li;
+            const unsigned at = (unsigned)(col < p.N ? col : p.N - 1) * fcol + (unsigned)r * fr;
+            if constexpr (F == PJ_F_RANKS) fv[j].v = *(const pj_u32x4*)(r < p.rank ? f + at : (const T*)pj_zero16);
+            else
+#pragma unroll
+                for (int u = 0; u < V; ++u) fv[j].t[u] = r + u < p.rank ? f[at + (unsigned)u * fr] : (T)0;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int u = 0; u < NP; ++u) hv[i][u] = *(const pj_u32x4*)(h + (long long)i * 16 * (NP * rp) + u * rp + q + lh * V);
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+#pragma unroll
+                for (int u = NP - 1; u >= 0; --u) acc[i][j] = pj_mfma<DT>(fv[j].v, hv[i][u], acc[i][j]);
+    }
+    if constexpr (DT == VDB_F16)
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const float sc = p.h_scale[row + i * 16 + li];
+#pragma unroll
+            for (int j = 0; j < C; ++j) acc[i][j] = acc[i][j] * sc;
+        }
+}
+
 // Every lane its own row's adapter: t += h[m] f[a]^T for its four columns of each block, ranks q0, q0 + qs, ... in steps of V
 template <int DT, int F, int C>
 __device__ __forceinline__ void pj_low_rank_lanes(const ProjRows& p, long long mc, int colb, int a, int q0, int qs, pj_f32x4 (&t)[C]) {
@@ -407,7 +514,7 @@ __device__ __forceinline__ void pj_low_rank_lanes(const ProjRows& p, long long m
     const unsigned fr = (unsigned)p.f_rank, fcol = (unsigned)p.f_col;
     const T* f = (const T*)p.f + (long long)(a < 0 ? 0 : a) * p.f_adapter;
     const T* h = (const T*)p.h + mc * (NP * rp);
-#pragma unroll 1
+#pragma unroll F == PJ_F_RANKS ? 2 : 1
     for (int q = q0; q < p.rank; q += qs) {
         float hq[V] = {};
 #pragma unroll
@@ -464,6 +571,17 @@ __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, in
                                             int waves = 1, int wave = 0) {
     constexpr int V = 16 / PJ<DT>::E;
     const int li = threadIdx.x & 15;
+    if constexpr (B > 1 && F != PJ_F_ANY) {
+        // one adapter for all rows, as long requests have it: its factor is loaded once for all of them
+        const int a0 = __builtin_amdgcn_readlane(am[0], 0);
+        bool same = a0 >= 0;
+#pragma unroll
+        for (int i = 0; i < B; ++i) same = same && am[i] == a0;
+        if (__ballot(!same) == 0) {
+            pj_low_rank_all<DT, F, B, C>(p, row, colb, a0, acc);
+            return;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < B; ++i) {
         const long long m = row + i * 16 + li, mc = m < p.n ? m : p.n - 1;
@@ -499,8 +617,28 @@ __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, in
 struct PJRowsArgs {
     ProjRows p;
     int col_tiles;
-    bool vec_out;
+    bool vec_out;                // y can be written in aligned pieces of 16 bytes
 };
+
+// The tile of `tm` rows that this workgroup works on: rows [max(row0, first), min(row0 + tm, row1)); false: none.
+template <bool ADAPT>
+__device__ __forceinline__ bool pj_place(const ProjRows& p, int tm, int col_tiles, int& seg, long long& row0, long long& first,
+                                         long long& row1, int& col) {
+    if constexpr (!ADAPT) return pj_find_tile(p.offsets, p.segments, p.n, tm, col_tiles, blockIdx.x, seg, row0, row1, col);
+    else {
+        // one matrix for all rows: tiles over the rows from the first segment's start to the last one's end
+        first = pj_clamp(p.offsets[0], p.n);
+        row1 = pj_clamp(p.offsets[p.segments], p.n);
+        if (row1 <= first) return false;
+        const long long t0 = first / tm, tiles = (row1 + tm - 1) / tm - t0;
+        const long long all = tiles * col_tiles, run = (all + 7) / 8, idx = blockIdx.x >> 3;
+        const long long id = (long long)(blockIdx.x & 7) * run + idx;
+        if (idx >= run || id >= all) return false;
+        col = (int)(id % col_tiles);
+        row0 = (t0 + id / col_tiles) * tm;
+        return true;
+    }
+}
 
 template <int DT, int ODT, bool NK, bool VEC, bool ADAPT, int F, int R>
 __global__ void __launch_bounds__(PJ_THREADS, 2)
@@ -513,20 +651,7 @@ proj_rows_kernel(PJRowsArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     long long row0, row1, first = 0;         // rows of this tile: [max(row0, first), row1)
     int seg = 0, col;
-    if constexpr (ADAPT) {
-        // one matrix for all rows: tiles over the rows from the first segment's start to the last one's end
-        const long long begin = pj_clamp(p.offsets[0], p.n), end = pj_clamp(p.offsets[p.segments], p.n);
-        if (end <= begin) return;
-        const long long t0 = begin / R, tiles = (end + R - 1) / R - t0;
-        const long long all = tiles * a.col_tiles, run = (all + 7) / 8, idx = blockIdx.x >> 3;
-        const long long id = (long long)(blockIdx.x & 7) * run + idx;
-        if (idx >= run || id >= all) return;
-        col = (int)(id % a.col_tiles);
-        row0 = (t0 + id / a.col_tiles) * R;
-        first = begin; row1 = end;
-    } else {
-        if (!pj_find_tile(p.offsets, p.segments, p.n, R, a.col_tiles, blockIdx.x, seg, row0, row1, col)) return;
-    }
+    if (!pj_place<ADAPT>(p, R, a.col_tiles, seg, row0, first, row1, col)) return;
     const int col0 = col * R;
     pj_f32x4 acc[B][B] = {};
     PJProduct<DT, false, NK, VEC, R> prod;
@@ -537,6 +662,31 @@ proj_rows_kernel(PJRowsArgs a) {
     prod.begin(p.K, pj_lds);
     if constexpr (ADAPT) pj_low_rank<DT, F, B, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), am, acc);
     prod.run(pj_lds, wm, wn, acc);
+    if (R == 128 && a.vec_out && row0 >= first && row0 + R <= row1 && col0 + R <= p.N) {
+        // A lane holds four columns of a row: stored as they are, a wave's store would be sixteen pieces of 32 or 64 bytes.  Turned
+        // in LDS it is four or eight rows of whole cache lines (65 536 x 768 rows out: 112 -> 99 us bf16, 167 -> 157 us fp32).
+        typedef typename PJ<ODT>::T O;
+        __syncthreads();                                     // the ring is free; from here each wave has a quarter of it
+        constexpr int LINE = (R / 2) * PJ<ODT>::E + 16, LPR = (LINE - 16) / 16, RPI = 64 / LPR;      // lanes to a row, rows to a store
+        constexpr int BI = ODT == VDB_F32 ? B / 2 : B;       // blocks of 16 rows that fit
+        static_assert(BI * 16 * LINE <= PJRing<R>::BYTES / 4, "a wave's part of the ring");
+        char* const mine = pj_lds + wave * (PJRing<R>::BYTES / 4);
+        O* const y = (O*)p.y + (row0 + wm * (R / 2)) * p.ldy + col0 + wn * (R / 2);
+#pragma unroll
+        for (int h = 0; h < B; h += BI) {
+#pragma unroll
+            for (int i = 0; i < BI; ++i)
+#pragma unroll
+                for (int j = 0; j < B; ++j)
+                    pj_store4<ODT>(mine + (i * 16 + li) * LINE + (j * 16 + lh * 4) * PJ<ODT>::E, 0, acc[h + i][j], 4);
+#pragma unroll
+            for (int r = 0; r < BI * 16; r += RPI) {
+                const pj_u32x4 v = *(const pj_u32x4*)(mine + (r + lane / LPR) * LINE + lane % LPR * 16);
+                *(pj_u32x4*)((char*)(y + (h * 16 + r + lane / LPR) * p.ldy) + lane % LPR * 16) = v;
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < B; ++i) {
         const long long m = row0 + wm * (R / 2) + i * 16 + li;
@@ -544,7 +694,7 @@ proj_rows_kernel(PJRowsArgs a) {
 #pragma unroll
         for (int j = 0; j < B; ++j) {
             const int c = col0 + wn * (R / 2) + j * 16 + lh * 4;
-            if (c < p.N) pj_store4<ODT>(p.y, m * p.ldy + c, acc[i][j], p.N - c, a.vec_out);
+            if (c < p.N) pj_store4<ODT>(p.y, m * p.ldy + c, acc[i][j], p.N - c);
         }
     }
 }
@@ -587,13 +737,12 @@ proj_few_kernel(PJRowsArgs a) {
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * 4 * KS + lh * V;
             if constexpr (VEC) xa[u].v = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
-            else
-#pragma unroll
-                for (int j = 0; j < V; ++j) xa[u].t[j] = k + j < p.K ? x[k + j] : (T)0;
+            else xa[u].v = pj_piece<T>(x + k, p.K - k);
             if constexpr (VEC && !NK) wa[u].v = *(const pj_u32x4*)(k < p.K ? w + k : (const T*)pj_zero16);
+            else if constexpr (!NK) wa[u].v = pj_piece<T>(w + k, p.K - k);
             else
 #pragma unroll
-                for (int j = 0; j < V; ++j) wa[u].t[j] = k + j < p.K ? w[NK ? (k + j) * p.ldw : (long long)(k + j)] : (T)0;
+                for (int j = 0; j < V; ++j) wa[u].t[j] = k + j < p.K ? w[(k + j) * p.ldw] : (T)0;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) acc[0][0] = pj_mfma<DT>(wa[u].v, xa[u].v, acc[0][0]);
@@ -607,16 +756,17 @@ proj_few_kernel(PJRowsArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += part[i][lane][j];
     const int cs = col * 16 + lh * 4;
-    if (m < row1 && m >= first && cs < p.N) pj_store4<ODT>(p.y, m * p.ldy + cs, v, p.N - cs, a.vec_out);
+    if (m < row1 && m >= first && cs < p.N) pj_store4<ODT>(p.y, m * p.ldy + cs, v, p.N - cs);
 }
 
 struct PJWeightsArgs {
     ProjWeights p;
     int m_tiles, n_tiles;
-    bool vec_out;
 };
 
-template <int DT, int ODT, bool VEC, int R>
+// dw of one segment, or of one chunk of its rows (SPLIT: a segment of more than one chunk leaves fp32 partial sums, which
+// proj_weights_sum_kernel adds up in the order of the chunks).
+template <int DT, int ODT, bool VEC, bool SPLIT, int R>
 __global__ void __launch_bounds__(PJ_THREADS, 2)
 proj_weights_kernel(PJWeightsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char pj_lds[];
@@ -625,9 +775,21 @@ proj_weights_kernel(PJWeightsArgs a) {
     const ProjWeights& p = a.p;
     const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-    const int seg = blockIdx.x / (a.m_tiles * a.n_tiles), rest = blockIdx.x % (a.m_tiles * a.n_tiles);
-    const int m0 = rest / a.n_tiles * R, n0 = rest % a.n_tiles * R;
-    const long long b = pj_clamp(p.offsets[seg], p.n), e = pj_clamp(p.offsets[seg + 1], p.n);
+    int seg, tile;
+    long long b, e, item = -1;               // rows; number of the chunk, -1: the whole segment
+    if constexpr (SPLIT) {
+        if (!pj_find_tile(p.offsets, p.segments, p.n, p.chunk, a.m_tiles * a.n_tiles, blockIdx.x, seg, b, e, tile, item)) return;
+        if (item >= p.n / p.chunk + p.segments) return;       // offsets that decrease: more chunks than the workspace holds
+        const long long sb = pj_clamp(p.offsets[seg], p.n);
+        if (b == sb && e - b <= p.chunk) item = -1;
+        e = e - b < p.chunk ? e : b + p.chunk;
+    } else {
+        seg = blockIdx.x / (a.m_tiles * a.n_tiles);
+        tile = blockIdx.x % (a.m_tiles * a.n_tiles);
+        b = pj_clamp(p.offsets[seg], p.n);
+        e = pj_clamp(p.offsets[seg + 1], p.n);
+    }
+    const int m0 = tile / a.n_tiles * R, n0 = tile % a.n_tiles * R;
     pj_f32x4 acc[B][B] = {};
     PJProduct<DT, true, true, VEC, R> prod;
     prod.om.init((const T*)p.dy + b * p.lddy, p.lddy, m0, p.M);
@@ -641,7 +803,9 @@ proj_weights_kernel(PJWeightsArgs a) {
 #pragma unroll
         for (int j = 0; j < B; ++j) {
             const int c = n0 + wn * (R / 2) + j * 16 + lh * 4;
-            if (c < p.N) pj_store4<ODT>(p.dw, ((long long)seg * p.M + m) * p.N + c, acc[i][j], p.N - c, a.vec_out);
+            if (c >= p.N) continue;
+            if (SPLIT && item >= 0) pj_store4<VDB_F32>(p.partial, (item * p.M + m) * p.N + c, acc[i][j], p.N - c);
+            else pj_store4<ODT>(p.dw, ((long long)seg * p.M + m) * p.N + c, acc[i][j], p.N - c);
         }
     }
 }
@@ -673,7 +837,7 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     a.p = p;
     a.col_tiles = (p.N + R - 1) / R;
     constexpr int E = PJ<DT>::E, V = 16 / E;
-    a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 4 * PJ<ODT>::E);
+    a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 16);
     const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + p.segments;
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const size_t lds = PJRing<R>::BYTES;
@@ -702,7 +866,7 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
     a.p = p;
     a.col_tiles = (p.N + 15) / 16;
     constexpr int V = 16 / PJ<DT>::E;
-    a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 4 * PJ<ODT>::E);
+    a.vec_out = false;
     const long long row_tiles = p.row_adapter ? (p.n + 15) / 16 : p.n / 16 + p.segments;
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const bool fv = pj_factor_vec<DT, V>(p);
@@ -737,19 +901,24 @@ static hipError_t pj_weights_sized(const ProjWeights& p, bool vec, hipStream_t s
     a.p = p;
     a.m_tiles = (p.M + R - 1) / R;
     a.n_tiles = (p.N + R - 1) / R;
-    a.vec_out = pj_aligned(p.dw, p.N, PJ<ODT>::E, 4 * PJ<ODT>::E);
     const dim3 grid((unsigned)((long long)p.segments * a.m_tiles * a.n_tiles));
-    if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, R>, grid, PJRing<R>::BYTES, a, st);
-    else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, R>, grid, PJRing<R>::BYTES, a, st)
-                    : pj_launch(proj_weights_kernel<DT, ODT, false, R>, grid, PJRing<R>::BYTES, a, st);
+    const size_t lds = PJRing<R>::BYTES;
+    if (p.chunk > 0) {
+        const dim3 chunks((unsigned)(((p.n / p.chunk + p.segments) * a.m_tiles * a.n_tiles + 7) / 8 * 8));
+        if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st);
+        else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st)
+                        : pj_launch(proj_weights_kernel<DT, ODT, false, true, R>, chunks, lds, a, st);
+    }
+    if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, false, R>, grid, lds, a, st);
+    else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, false, R>, grid, lds, a, st)
+                    : pj_launch(proj_weights_kernel<DT, ODT, false, false, R>, grid, lds, a, st);
 }
 
 template <int DT, int ODT>
 static hipError_t pj_weights(const ProjWeights& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool vec = pj_aligned(p.dy, p.lddy, E, 16) && pj_aligned(p.x, p.ldx, E, 16) && p.M % V == 0 && p.N % V == 0;
-    const long long tiles = (long long)p.segments * ((p.M + 127) / 128) * ((p.N + 127) / 128);
-    return vec && !pj_small_tiles(tiles) ? pj_weights_sized<DT, ODT, 128>(p, vec, st) : pj_weights_sized<DT, ODT, 64>(p, vec, st);
+    return vec && p.tile == 128 ? pj_weights_sized<DT, ODT, 128>(p, vec, st) : pj_weights_sized<DT, ODT, 64>(p, vec, st);
 }
 
 // A type's rows and weights products; defined in kernels_project_{f32,bf16,f16}.hip.

@@ -2105,7 +2105,11 @@ struct ProjWork {
 };
 
 static int64_t proj_workspace(const vdb_projection* p, int64_t n, bool adapted, bool backward) {
-    return adapted ? ProjWork(p, n, backward).all : 0;
+    if (adapted) return ProjWork(p, n, backward).all;
+    if (!backward) return 0;
+    int tile, chunk;
+    proj_weights_plan(n, p->groups, (int)p->dim_out, (int)p->dim_in, tile, chunk);
+    return chunk > 0 ? (n / chunk + p->groups) * p->dim_out * p->dim_in * (int64_t)sizeof(float) : 0;
 }
 
 static int workspace_check(void* ws, int64_t have, int64_t want) {
@@ -2192,7 +2196,11 @@ int vdb_project_grouped_backward_dev(const vdb_projection* p, int64_t n, const v
     }
     if (dw && (blocks_overlap(dw, dwb, p->w, wn * rx.esize()) || blocks_overlap(dw, dwb, offsets, (p->groups + 1) * (int64_t)8)))
         return fail(VDB_EINVAL, "dw shares memory with an input");
-    if ((rc = workspace_check(workspace, workspace_bytes, proj_workspace(p, n, false, true)))) return rc;
+    const int64_t want = dw ? proj_workspace(p, n, false, true) : 0;
+    if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
+    if (want > 0 && (block_overlap(workspace, want, rdy, n) || block_overlap(workspace, want, rx, n) || (dx && block_overlap(workspace, want, rdx, n)) ||
+                     blocks_overlap(workspace, want, dw, dwb) || blocks_overlap(workspace, want, p->w, wn * rx.esize())))
+        return fail(VDB_EINVAL, "the workspace shares memory with another argument");
     if ((rc = enter())) return rc;
     hipStream_t st = (hipStream_t)stream;
     if (dx && n > 0) {
@@ -2204,7 +2212,10 @@ int vdb_project_grouped_backward_dev(const vdb_projection* p, int64_t n, const v
         ProjWeights w{};
         w.dy = dy; w.lddy = lddy; w.x = x; w.ldx = ldx; w.dw = dw; w.M = (int)p->dim_out; w.N = (int)p->dim_in;
         w.n = n; w.dtype = p->dtype; w.out_dtype = p->out_dtype; w.offsets = (const long long*)offsets; w.segments = p->groups;
+        proj_weights_plan(n, p->groups, w.M, w.N, w.tile, w.chunk);
+        w.partial = (float*)workspace;
         VDB_HIP(launch_proj_weights(w, st));
+        if (w.chunk > 0) VDB_HIP(launch_proj_weights_sum(w, st));
     }
     return VDB_OK;
 }
