@@ -217,6 +217,16 @@ proj_shrink_kernel(ProjShrink p, int share) {
     pj_shrink_block<DT, NRB, XV, F>(p, (long long)(blockIdx.x / share) * 16, blockIdx.x % share, share, smem);
 }
 
+// Both intermediates of a backward pass in one launch: g of dy (its factor contiguous along the ranks), h of x.
+template <int DT, int NRB>
+__global__ void __launch_bounds__(256)
+proj_shrink_pair_kernel(ProjShrink g, ProjShrink h, int share) {
+    __shared__ __attribute__((aligned(16))) char smem[pj_shrink_block_lds<DT, NRB, PJ_S_FR>()];
+    const long long r0 = (long long)(blockIdx.x / share) * 16;
+    if (blockIdx.y == 0) pj_shrink_block<DT, NRB, true, PJ_S_FR>(g, r0, blockIdx.x % share, share, smem);
+    else pj_shrink_block<DT, NRB, true, PJ_S_FK>(h, r0, blockIdx.x % share, share, smem);
+}
+
 // Many rows of long requests: 64 rows by all ranks through LDS, a ring of four stages of 128 bytes of k as in PJProduct, each
 // wave 16 rows.  For every adapter of the 64 rows (up to four) the whole product; 64 rows of more adapters are left to the
 // workgroups behind the first `tiles`, which take 16 rows each as above and have nothing to do otherwise.
@@ -336,9 +346,12 @@ template <int DT, int NRB, bool XV> struct PJFactorRows {
     }
 };
 
+// blockIdx.z: the gradient of A, of B.
 template <int DT, int ODT, int NRB, bool XV>
 __global__ void __launch_bounds__(PJ_FACTOR_WAVES * 64)
-proj_factor_kernel(ProjFactor p) {
+proj_factor_kernel(ProjFactor pa, ProjFactor pb) {
+    const ProjFactor& p = blockIdx.z == 0 ? pa : pb;
+    if ((int)blockIdx.x * 64 >= p.N) return;
     typedef typename PJ<ODT>::T O;
     constexpr int W = PJ_FACTOR_WAVES;
     __shared__ pj_f32x4 part[W - 1][4][64];
@@ -468,22 +481,35 @@ hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st) {
     return pj_launch(proj_weights_sum_kernel<VDB_F16>, grid, 0, p, st);
 }
 
-// Rows, and average length of a request, from which the shrink works by 64 rows.
+// Workgroups for the adapters of one block of 16 rows: as many as it meets if all requests were of one length, and a workgroup to
+// a CU.  More are dispatched in vain (1024 rows of 128 requests: 12.4 us with 256 workgroups in all, 15.1 with 1024), fewer
+// leave adapters one after the other (15.8 us with 128).
+static long long shrink_share(long long n, int segments) {
+    const long long blocks = (n + 15) / 16;
+    long long share = segments / blocks;
+    if (share < 256 / blocks) share = 256 / blocks;
+    if (share > segments) share = segments;
+    return share < 1 ? 1 : share > 16 ? 16 : share;
+}
+
+// By 64 rows: from rank 33 and 16 384 rows on, for long requests (rank 64, 1024 wide, 48 requests: 32 768 rows 47 -> 26 us, 8192 rows
+// 22 -> 30; rank 16, 768 wide: 16 384 rows 12 -> 17).
 #ifndef PJ_SHRINK_TILE_ROWS
-#define PJ_SHRINK_TILE_ROWS 8192
+#define PJ_SHRINK_TILE_ROWS 16384
 #endif
-#ifndef PJ_SHRINK_TILE_LEN
-#define PJ_SHRINK_TILE_LEN 128
-#endif
+template <int DT, int NRB> static bool shrink_tiles(const ProjShrink& p) {
+    return NRB >= 4 && p.n >= PJ_SHRINK_TILE_ROWS && p.n / p.segments >= 128;
+}
+
 template <int DT, int NRB>
 static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool xv = pj_aligned(p.x, p.ldx, E, 16) && p.K % V == 0;
     const bool fk = p.f_k == 1 && pj_aligned(p.f, p.f_rank, E, 16) && p.K % V == 0;
     const bool ftile = p.f_rank == 1 && p.f_k == p.rank && p.rank % V == 0 && (uintptr_t)p.f % 16 == 0;
-    const bool fr = DT != VDB_F32 && p.f_rank == 1 && p.f_k == p.rank && p.rank % 8 == 0 && (uintptr_t)p.f % 16 == 0;
+    const bool fr = DT == VDB_F32 ? p.f_rank == 1 : p.f_rank == 1 && p.f_k == p.rank && p.rank % 8 == 0 && (uintptr_t)p.f % 16 == 0;
     const long long blocks = (p.n + 15) / 16;
-    if (p.n >= PJ_SHRINK_TILE_ROWS && p.n / p.segments >= PJ_SHRINK_TILE_LEN && xv && (fk || ftile)) {
+    if constexpr (NRB >= 4) if (shrink_tiles<DT, NRB>(p) && xv && (fk || ftile)) {
         const int tiles = (int)((p.n + 63) / 64);
         const dim3 grid((unsigned)(tiles + blocks));
         const size_t lds = 4 * (pj_tile_bytes(64) + pj_tile_bytes(NRB <= 4 ? 64 : 128));
@@ -498,29 +524,25 @@ static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
         if (fk) return go(proj_shrink_tile_kernel<DT, NRB, PJ_S_FK>);
         return go(proj_shrink_tile_kernel<DT, NRB, PJ_S_FR>);
     }
-    // workgroups for the adapters of one block: as many as it meets if all requests were of one length, and a workgroup to a CU.
-    // More are dispatched in vain (1024 rows of 128 requests: 12.4 us with 256 workgroups in all, 15.1 with 1024), fewer leave
-    // adapters one after the other (15.8 us with 128).
-    long long share = (long long)p.segments / blocks;
-    if (share < 256 / blocks) share = 256 / blocks;
-    if (share > p.segments) share = p.segments;
-    share = share < 1 ? 1 : share > 16 ? 16 : share;
+    const long long share = shrink_share(p.n, p.segments);
     const dim3 grid((unsigned)(blocks * share));
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, (int)share);
         return hipGetLastError();
     };
     if (!xv || !(fk || fr)) return go(proj_shrink_kernel<DT, NRB, false, PJ_S_ANY>);
-    if constexpr (DT != VDB_F32) if (!fk) return go(proj_shrink_kernel<DT, NRB, true, PJ_S_FR>);
+    if (!fk) return go(proj_shrink_kernel<DT, NRB, true, PJ_S_FR>);
     return go(proj_shrink_kernel<DT, NRB, true, PJ_S_FK>);
 }
 
 template <int DT, int ODT, int NRB>
-static hipError_t factor_typed(const ProjFactor& p, hipStream_t st) {
-    const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)p.adapters), threads(PJ_FACTOR_WAVES * 64);
-    const bool xv = pj_aligned(p.x, p.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && p.N % 4 == 0;
-    if (xv) hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, true>), grid, threads, 0, st, p);
-    else hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, false>), grid, threads, 0, st, p);
+static hipError_t factor_typed(const ProjFactor& p, const ProjFactor& b, hipStream_t st) {
+    const int most = p.N > b.N ? p.N : b.N;
+    const dim3 grid((unsigned)((most + 63) / 64), (unsigned)p.adapters, 2), threads(PJ_FACTOR_WAVES * 64);
+    const bool xv = pj_aligned(p.x, p.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && p.N % 4 == 0 &&
+                    pj_aligned(b.x, b.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && b.N % 4 == 0;
+    if (xv) hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, true>), grid, threads, 0, st, p, b);
+    else hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, false>), grid, threads, 0, st, p, b);
     return hipGetLastError();
 }
 
@@ -543,14 +565,38 @@ hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st) {
 #undef PJ_SHRINK
 }
 
-hipError_t launch_proj_factor(const ProjFactor& p, hipStream_t st) {
-    if (p.dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_F32, VDB_F32, NRB>(p, st)));
-    if (p.dtype == VDB_BF16) {
-        if (p.out_dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_BF16, VDB_F32, NRB>(p, st)));
-        PJ_BY_RANK(return (factor_typed<VDB_BF16, VDB_BF16, NRB>(p, st)));
+template <int DT, int NRB>
+static hipError_t shrink_pair_typed(const ProjShrink& g, const ProjShrink& h, hipStream_t st) {
+    constexpr int E = PJ<DT>::E, V = 16 / E;
+    const bool vec = pj_aligned(g.x, g.ldx, E, 16) && g.K % V == 0 && pj_aligned(h.x, h.ldx, E, 16) && pj_aligned(h.f, h.f_rank, E, 16) &&
+                     h.K % V == 0 && (DT == VDB_F32 || (g.rank % 8 == 0 && (uintptr_t)g.f % 16 == 0));
+    if (!vec || shrink_tiles<DT, NRB>(g)) {
+        const hipError_t e = shrink_typed<DT, NRB>(g, st);
+        return e == hipSuccess ? shrink_typed<DT, NRB>(h, st) : e;
     }
-    if (p.out_dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_F16, VDB_F32, NRB>(p, st)));
-    PJ_BY_RANK(return (factor_typed<VDB_F16, VDB_F16, NRB>(p, st)));
+    const long long share = shrink_share(g.n, g.segments);
+    const dim3 grid((unsigned)((g.n + 15) / 16 * share), 2);
+    hipLaunchKernelGGL((proj_shrink_pair_kernel<DT, NRB>), grid, dim3(256), 0, st, g, h, (int)share);
+    return hipGetLastError();
+}
+
+hipError_t launch_proj_shrink_pair(const ProjShrink& g, const ProjShrink& h, hipStream_t st) {
+    if (g.n <= 0 || g.segments <= 0) return hipSuccess;
+    if (g.dtype == VDB_F32) { const ProjShrink& p = g; PJ_BY_RANK(return (shrink_pair_typed<VDB_F32, NRB>(g, h, st))); }
+    const int nrb = proj_rank_pad(g.rank, g.dtype) / 16;
+#define PJ_PAIR(DT) (nrb <= 2 ? shrink_pair_typed<DT, 2>(g, h, st) : nrb <= 4 ? shrink_pair_typed<DT, 4>(g, h, st) : shrink_pair_typed<DT, 8>(g, h, st))
+    return g.dtype == VDB_BF16 ? PJ_PAIR(VDB_BF16) : PJ_PAIR(VDB_F16);
+#undef PJ_PAIR
+}
+
+hipError_t launch_proj_factors(const ProjFactor& p, const ProjFactor& b, hipStream_t st) {
+    if (p.dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_F32, VDB_F32, NRB>(p, b, st)));
+    if (p.dtype == VDB_BF16) {
+        if (p.out_dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_BF16, VDB_F32, NRB>(p, b, st)));
+        PJ_BY_RANK(return (factor_typed<VDB_BF16, VDB_BF16, NRB>(p, b, st)));
+    }
+    if (p.out_dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_F16, VDB_F32, NRB>(p, b, st)));
+    PJ_BY_RANK(return (factor_typed<VDB_F16, VDB_F16, NRB>(p, b, st)));
 }
 
 hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st) {

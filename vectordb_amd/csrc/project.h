@@ -94,7 +94,9 @@ hipError_t launch_proj_weights_f16(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st);
 hipError_t launch_proj_weights(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st);      // the second step where segments are split
-hipError_t launch_proj_factor(const ProjFactor& p, hipStream_t st);
+// both intermediates of a backward pass, of dy and of x; the gradients of both factors
+hipError_t launch_proj_shrink_pair(const ProjShrink& g, const ProjShrink& h, hipStream_t st);
+hipError_t launch_proj_factors(const ProjFactor& a, const ProjFactor& b, hipStream_t st);
 // rows [n, dim] of q outside every segment become zero
 hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st);
 

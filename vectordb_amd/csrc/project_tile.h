@@ -331,6 +331,7 @@ template <int N> __device__ __forceinline__ void pj_wait_and_meet() {
 template <int R> struct PJRing {
     static constexpr int STAGES = R == 64 ? 4 : 2;
     static constexpr int BYTES = STAGES * 2 * pj_tile_bytes(R);
+    static constexpr int HALVES = 2 * 2 * pj_tile_bytes(R);          // through registers: two stages
 };
 
 // One R x R output tile: a ring of LDS stages, each the next 128 bytes of k of both operands.  The loads of a stage are
@@ -418,9 +419,10 @@ struct PJProduct {
 // The term h f^T of a wave's block, before the main product.  The fp32 intermediate h comes in parts of the rows' type that add up
 // to it (bf16: three; fp16: two, with a power of two for each row that brings its largest entry to 1/2..1, as fp16 could
 // not hold it), so that neither way below rounds h:
-//   up to two adapters in 16 rows: the matrix unit, all 16 rows by one adapter, taken over by the rows of that adapter only,
-//     so that what one adapter holds never reaches another request's rows;
-//   more: every lane for itself, its row by its four columns, which waits once for all adapters instead of once for each.
+//   few adapters in 16 rows (two, or one for each 12 ranks): the matrix unit, all 16 rows by one adapter, taken over by the
+//     rows of that adapter only, so that what one adapter holds never reaches another request's rows;
+//   more: every lane for itself, its row by its four columns, which waits once for all adapters instead of once for each, in a time
+//     that grows with the rank.
 
 // How the factor f lies: entry (column, rank) of an adapter at column * f_col + rank * f_rank elements (32 bits hold it).
 //   PJ_F_RANKS   ranks contiguous, 16-byte pieces of them aligned (B of a forward pass)
@@ -585,23 +587,23 @@ __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, in
 #pragma unroll
     for (int i = 0; i < B; ++i) {
         const long long m = row + i * 16 + li, mc = m < p.n ? m : p.n - 1;
-        unsigned left = (unsigned)__ballot(am[i] >= 0) & 0xffffu;
-        if (!left) continue;
-        const int a0 = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
-        left &= ~(unsigned)__ballot(am[i] == a0);
-        int a1 = -1;
-        if (left) {
-            a1 = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
-            left &= ~(unsigned)__ballot(am[i] == a1);
-        }
+        const unsigned rows = (unsigned)__ballot(am[i] >= 0) & 0xffffu;
+        if (!rows) continue;
+        int met = 0;                                         // adapters in these 16 rows
+        for (unsigned left = rows; left; ++met) left &= ~(unsigned)__ballot(am[i] == __builtin_amdgcn_readlane(am[i], __builtin_ctz(left)));
         pj_f32x4 t[C] = {};
-        if (!left) {
-            if (wave == 0) pj_low_rank_block<DT, F, C>(p, mc, colb, a0, t);
-            if (a1 >= 0) {
-                pj_f32x4 t1[C] = {};
-                if (wave == waves - 1) pj_low_rank_block<DT, F, C>(p, mc, colb, a1, t1);
+        if (met <= (p.rank < 32 ? 2 : p.rank / 12)) {
+            int turn = 0;
+            for (unsigned left = rows; left;) {
+                const int ad = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
+                left &= ~(unsigned)__ballot(am[i] == ad);
+                const bool mine = turn == wave;
+                turn = turn + 1 == waves ? 0 : turn + 1;
+                if (!mine) continue;
+                pj_f32x4 u[C] = {};
+                pj_low_rank_block<DT, F, C>(p, mc, colb, ad, u);
 #pragma unroll
-                for (int j = 0; j < C; ++j) if (am[i] == a1) t[j] = t1[j];
+                for (int j = 0; j < C; ++j) if (am[i] == ad) t[j] = u[j];
             }
         } else {
             pj_low_rank_lanes<DT, F, C>(p, mc, colb, am[i], wave * V, waves * V, t);
@@ -840,7 +842,7 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 16);
     const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + p.segments;
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
-    const size_t lds = PJRing<R>::BYTES;
+    const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
     const bool fv = pj_factor_vec<DT, V>(p);
 #define PJ_ROWS(NK, VEC)                                                                              \
     (!p.row_adapter ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY, R>, grid, lds, a, st)     \
@@ -902,7 +904,7 @@ static hipError_t pj_weights_sized(const ProjWeights& p, bool vec, hipStream_t s
     a.m_tiles = (p.M + R - 1) / R;
     a.n_tiles = (p.N + R - 1) / R;
     const dim3 grid((unsigned)((long long)p.segments * a.m_tiles * a.n_tiles));
-    const size_t lds = PJRing<R>::BYTES;
+    const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
     if (p.chunk > 0) {
         const dim3 chunks((unsigned)(((p.n / p.chunk + p.segments) * a.m_tiles * a.n_tiles + 7) / 8 * 8));
         if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st);

@@ -2291,12 +2291,14 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     s.f = p->b; s.f_adapter = p->dim_out * p->rank; s.f_rank = 1; s.f_k = p->rank;
     s.row_adapter = dx ? (int*)ws : nullptr; s.h = dx ? ws + wk.rows : nullptr; s.h_scale = (float*)(ws + wk.rows + wk.parts);
     s.h32 = da ? g32 : nullptr;
-    VDB_HIP(launch_proj_shrink(s, st));
     if (da) {
         // h = s x A^T, again rather than kept from the forward pass
-        s.x = x; s.ldx = ldx; s.K = (int)p->dim_in;
-        s.f = p->a; s.f_adapter = p->rank * p->dim_in; s.f_rank = p->dim_in; s.f_k = 1;
-        s.row_adapter = nullptr; s.h = nullptr; s.h_scale = nullptr; s.h32 = h32;
+        ProjShrink t = s;
+        t.x = x; t.ldx = ldx; t.K = (int)p->dim_in;
+        t.f = p->a; t.f_adapter = p->rank * p->dim_in; t.f_rank = p->dim_in; t.f_k = 1;
+        t.row_adapter = nullptr; t.h = nullptr; t.h_scale = nullptr; t.h32 = h32;
+        VDB_HIP(launch_proj_shrink_pair(s, t, st));
+    } else {
         VDB_HIP(launch_proj_shrink(s, st));
     }
     if (dx && n > 0) {
@@ -2311,9 +2313,9 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
         f.rp = wk.rp32; f.rank = p->rank; f.n = n; f.dtype = p->dtype; f.out_dtype = p->out_dtype;
         f.offsets = (const long long*)offsets; f.segments = (int)requests; f.ids = adapter_ids; f.adapters = p->adapters;
         f.h = g32; f.x = x; f.ldx = ldx; f.N = (int)p->dim_in; f.out = da; f.by_col = false;
-        VDB_HIP(launch_proj_factor(f, st));
-        f.h = h32; f.x = dy; f.ldx = lddy; f.N = (int)p->dim_out; f.out = db; f.by_col = true;
-        VDB_HIP(launch_proj_factor(f, st));
+        ProjFactor fb = f;
+        fb.h = h32; fb.x = dy; fb.ldx = lddy; fb.N = (int)p->dim_out; fb.out = db; fb.by_col = true;
+        VDB_HIP(launch_proj_factors(f, fb, st));
     }
     return VDB_OK;
 }
