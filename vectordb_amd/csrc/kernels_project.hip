@@ -308,6 +308,107 @@ proj_shrink_tile_kernel(ProjShrink p, int tiles) {
     }
 }
 
+// ------------------------------------------------------------------------------------------- a few adapted rows, in one launch
+// y = x W^T + s (x A^T) B^T for 16 rows by 16 columns per workgroup, where there are so few rows that a second launch costs more
+// than what is done again here: every column tile makes its rows' h = s x A^T by itself (one product for each adapter that the 16
+// rows meet), the four waves over a quarter of the contracted axis each.  h stays in fp32, in LDS.
+// The rows and the matrix are loaded before the adapters are known; K is at most what that holds.
+template <int DT, int ODT, int NRB>
+__global__ void __launch_bounds__(256)
+proj_adapt_few_kernel(ProjRows p, ProjShrink s, int col_tiles) {
+    typedef typename PJ<DT>::T T;
+    constexpr int V = 16 / PJ<DT>::E, KS = 4 * V, XS = 8;
+    __shared__ pj_f32x4 part[4][NRB][64];
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4, wave = threadIdx.x >> 6;
+    const int c0 = (int)(blockIdx.x % col_tiles) * 16;
+    const long long r0 = (long long)(blockIdx.x / col_tiles) * 16, m = r0 + li;
+    const T* x = (const T*)p.x + (m < p.n ? m : p.n - 1) * p.ldx;
+    const T* w = (const T*)p.w + (long long)(c0 + li < p.N ? c0 + li : p.N - 1) * p.ldw;
+    pj_u32x4 xa[XS], wa[XS];
+    pj_shrink_load_x<DT, XS, true>(s, x, wave * KS, 4 * KS, xa);
+    pj_shrink_load_x<DT, XS, true>(s, w, wave * KS, 4 * KS, wa);
+    const long long first = pj_clamp(p.offsets[0], p.n), end = pj_clamp(p.offsets[p.segments], p.n);
+    int am[1];
+    pj_row_adapters<1>(s, r0, am);
+    // what this wave adds of the low-rank term: ranks wave * V.. of its row's factor, for its lanes' four columns
+    const int q = wave * V;
+    const bool some = am[0] >= 0 && q < p.rank;
+    const T* f = (const T*)p.f + (long long)(some ? am[0] : 0) * p.f_adapter;
+    union { T t[V]; pj_u32x4 v; } fv[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int col = c0 + lh * 4 + n;
+        fv[n].v = *(const pj_u32x4*)(some ? f + (unsigned)(col < p.N ? col : p.N - 1) * (unsigned)p.f_col + (unsigned)q : (const T*)pj_zero16);
+    }
+    const float sc = some ? (s.scale ? s.scale[am[0]] : 1.f) : 0.f;
+    // the adapters of the 16 rows one after the other, the factor of the next one on its way while one is multiplied
+    pj_f32x4 h[NRB] = {};
+    auto load = [&](int ad, pj_u32x4 (&fa)[XS][NRB]) __attribute__((always_inline)) {
+        const T* a = (const T*)s.f + (long long)ad * s.f_adapter;
+#pragma unroll
+        for (int u = 0; u < XS; ++u) {
+            const int k = wave * KS + u * 4 * KS + lh * V;
+#pragma unroll
+            for (int i = 0; i < NRB; ++i)
+                fa[u][i] = *(const pj_u32x4*)(k < s.K && i * 16 + li < s.rank ? a + (unsigned)(i * 16 + li) * (unsigned)s.f_rank + (unsigned)k : (const T*)pj_zero16);
+        }
+    };
+    pj_u32x4 fa[XS][NRB], fb[XS][NRB];
+    unsigned left = (unsigned)__ballot(am[0] >= 0) & 0xffffu;
+    int ad = left ? __builtin_amdgcn_readlane(am[0], __builtin_ctz(left)) : -1;
+    if (ad >= 0) load(ad, fa);
+    while (ad >= 0) {
+        left &= ~(unsigned)__ballot(am[0] == ad);
+        const int next = left ? __builtin_amdgcn_readlane(am[0], __builtin_ctz(left)) : -1;
+        if (next >= 0) load(next, fb);
+        pj_f32x4 t[NRB] = {};
+#pragma unroll
+        for (int u = 0; u < XS; ++u)
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) t[i] = pj_mfma<DT>(fa[u][i], xa[u], t[i]);
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) if (am[0] == ad) h[i] = t[i];
+#pragma unroll
+        for (int u = 0; u < XS; ++u)
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) fa[u][i] = fb[u][i];
+        ad = next;
+    }
+    pj_f32x4 acc = {};
+#pragma unroll
+    for (int u = 0; u < XS; ++u) acc = pj_mfma<DT>(wa[u], xa[u], acc);
+#pragma unroll
+    for (int i = 0; i < NRB; ++i) part[wave][i][lane] = h[i];
+    __syncthreads();
+    if (some) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            // ranks q + k.. of the lane's row: block (q + k) / 16, lane group (q + k) / 4 % 4
+            pj_f32x4 hv = {};
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                const pj_f32x4 t = part[o][(q + k) >> 4][((q + k) >> 2 & 3) * 16 + li];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) hv[j] += t[j];
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[n] = __builtin_fmaf(sc * hv[j], pj_to_f32<DT>(fv[n].t[k + j]), acc[n]);
+        }
+    }
+    __syncthreads();
+    if (wave) part[wave - 1][0][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int o = 0; o < 3; ++o)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += part[o][0][lane][j];
+    const int c = c0 + lh * 4;
+    if (m >= first && m < end && c < p.N) pj_store4<ODT>(p.y, m * p.ldy + c, acc, p.N - c);
+}
+
 // ------------------------------------------------------------------------------------------- gradient of the factors
 // One adapter's [rank] x 64 columns: the eight waves take its rows 16 at a time in turn, over every request that names the
 // adapter, and add up in wave order.  Products on the fp32 matrix unit: h is fp32, x is widened.
@@ -458,6 +559,16 @@ proj_zero_outside_kernel(float* q, long long dim, long long n, const long long* 
 }
 
 // ------------------------------------------------------------------------------------------- launches
+// input type x output type (the input's, or fp32)
+#define PJ_TYPES(dt, odt, CALL)                                                                              \
+    do {                                                                                                     \
+        if ((dt) == VDB_F32) { constexpr int DT = VDB_F32, ODT = VDB_F32; CALL; }                            \
+        else if ((dt) == VDB_BF16 && (odt) == VDB_F32) { constexpr int DT = VDB_BF16, ODT = VDB_F32; CALL; } \
+        else if ((dt) == VDB_BF16) { constexpr int DT = VDB_BF16, ODT = VDB_BF16; CALL; }                    \
+        else if ((odt) == VDB_F32) { constexpr int DT = VDB_F16, ODT = VDB_F32; CALL; }                      \
+        else { constexpr int DT = VDB_F16, ODT = VDB_F16; CALL; }                                            \
+    } while (0)
+
 #define PJ_BY_TYPE(FN)                                                              \
     do {                                                                            \
         if (p.dtype == VDB_F32) return FN##_f32(p, st);                             \
@@ -494,11 +605,8 @@ static long long shrink_share(long long n, int segments) {
 
 // By 64 rows: from rank 33 and 16 384 rows on, for long requests (rank 64, 1024 wide, 48 requests: 32 768 rows 47 -> 26 us, 8192 rows
 // 22 -> 30; rank 16, 768 wide: 16 384 rows 12 -> 17).
-#ifndef PJ_SHRINK_TILE_ROWS
-#define PJ_SHRINK_TILE_ROWS 16384
-#endif
 template <int DT, int NRB> static bool shrink_tiles(const ProjShrink& p) {
-    return NRB >= 4 && p.n >= PJ_SHRINK_TILE_ROWS && p.n / p.segments >= 128;
+    return NRB >= 4 && p.n >= 16384 && p.n / p.segments >= 128;
 }
 
 template <int DT, int NRB>
@@ -565,6 +673,29 @@ hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st) {
 #undef PJ_SHRINK
 }
 
+template <int DT, int ODT>
+static hipError_t adapt_few_typed(const ProjRows& p, const ProjShrink& s, hipStream_t st) {
+    const int col_tiles = (p.N + 15) / 16;
+    const dim3 grid((unsigned)((p.n + 15) / 16 * col_tiles));
+    constexpr int V = 16 / PJ<DT>::E;
+    if (p.rank <= 16 && p.rank <= 4 * V) hipLaunchKernelGGL((proj_adapt_few_kernel<DT, ODT, 1>), grid, dim3(256), 0, st, p, s, col_tiles);
+    else hipLaunchKernelGGL((proj_adapt_few_kernel<DT, ODT, 2>), grid, dim3(256), 0, st, p, s, col_tiles);
+    return hipGetLastError();
+}
+
+hipError_t launch_proj_adapted(const ProjRows& p, const ProjShrink& s, hipStream_t st) {
+    if (p.n <= 0 || p.segments <= 0) return hipSuccess;
+    const int e = p.dtype == VDB_F32 ? 4 : 2, v = 16 / e;
+    // One launch: up to 256 rows with no more than two requests to 16 of them, as the adapters of 16 rows are multiplied one after the
+    // other (768 x 768 bf16, rank 16, one launch against two: 1 row 5.1 and 8.5 us, 256 rows of one request 9.9 and 12.5, 512 rows
+    // 17.2 and 13.1; 64 rows of 8 requests 8.9 and 10.0, 64 rows of 64 requests 16.8 and 11.2).
+    const bool few = p.n <= 256 && p.segments <= 2 * ((p.n + 15) / 16) && p.K <= 512 / e * 4 && p.rank <= 4 * v && p.rank % v == 0 && p.K % v == 0 &&
+                     pj_aligned(p.x, p.ldx, e, 16) && pj_aligned(p.w, p.ldw, e, 16) && (uintptr_t)s.f % 16 == 0 && (uintptr_t)p.f % 16 == 0;
+    if (few) PJ_TYPES(p.dtype, p.out_dtype, return (adapt_few_typed<DT, ODT>(p, s, st)));
+    const hipError_t err = launch_proj_shrink(s, st);
+    return err == hipSuccess ? launch_proj_rows(p, st) : err;
+}
+
 template <int DT, int NRB>
 static hipError_t shrink_pair_typed(const ProjShrink& g, const ProjShrink& h, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
@@ -590,13 +721,7 @@ hipError_t launch_proj_shrink_pair(const ProjShrink& g, const ProjShrink& h, hip
 }
 
 hipError_t launch_proj_factors(const ProjFactor& p, const ProjFactor& b, hipStream_t st) {
-    if (p.dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_F32, VDB_F32, NRB>(p, b, st)));
-    if (p.dtype == VDB_BF16) {
-        if (p.out_dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_BF16, VDB_F32, NRB>(p, b, st)));
-        PJ_BY_RANK(return (factor_typed<VDB_BF16, VDB_BF16, NRB>(p, b, st)));
-    }
-    if (p.out_dtype == VDB_F32) PJ_BY_RANK(return (factor_typed<VDB_F16, VDB_F32, NRB>(p, b, st)));
-    PJ_BY_RANK(return (factor_typed<VDB_F16, VDB_F16, NRB>(p, b, st)));
+    PJ_TYPES(p.dtype, p.out_dtype, PJ_BY_RANK(return (factor_typed<DT, ODT, NRB>(p, b, st))));
 }
 
 hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st) {

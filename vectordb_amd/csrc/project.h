@@ -9,9 +9,9 @@
 namespace vdb {
 
 constexpr int PROJ_MAX_RANK = 128;
-#ifndef PJ_SPLIT_WGS
-#define PJ_SPLIT_WGS 768
-#endif
+// Workgroups that the gradient of the matrices is divided into where its output tiles are fewer (32 768 rows of 8 groups, 1024 x 768
+// bf16, whole backward pass: 287 us with 256, 206 with 512, 194 with 768, 204 with 1024).
+constexpr int PJ_SPLIT_WGS = 768;
 // A low-rank intermediate h [n, rank], fp32, is handed to the kernel that multiplies it as parts of the rows' type that add up
 // to it: rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks for 16-bit types, 16 for fp32).
 __host__ __device__ constexpr int proj_parts(int dtype) { return dtype == VDB_F32 ? 1 : dtype == VDB_BF16 ? 3 : 2; }
@@ -94,6 +94,8 @@ hipError_t launch_proj_weights_f16(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_shrink(const ProjShrink& p, hipStream_t st);
 hipError_t launch_proj_weights(const ProjWeights& p, hipStream_t st);
 hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st);      // the second step where segments are split
+// an adapted forward pass: the intermediate, then the rows, or both in one launch for a few rows
+hipError_t launch_proj_adapted(const ProjRows& p, const ProjShrink& s, hipStream_t st);
 // both intermediates of a backward pass, of dy and of x; the gradients of both factors
 hipError_t launch_proj_shrink_pair(const ProjShrink& g, const ProjShrink& h, hipStream_t st);
 hipError_t launch_proj_factors(const ProjFactor& a, const ProjFactor& b, hipStream_t st);

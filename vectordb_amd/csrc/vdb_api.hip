@@ -2144,12 +2144,10 @@ static hipError_t proj_adapted(const vdb_projection* p, int64_t n, const void* x
     s.scale = p->scale; s.rank = p->rank;
     s.row_adapter = (int*)ws; s.h = (char*)ws + wk.rows; s.h_scale = (float*)((char*)ws + wk.rows + wk.parts);
     s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = ids; s.adapters = p->adapters;
-    hipError_t e = launch_proj_shrink(s, st);
-    if (e != hipSuccess) return e;
     ProjRows r = proj_forward(p, n, x, ldx, offsets, requests, y, ldy, out_dtype);
     r.w_group = 0; r.row_adapter = s.row_adapter; r.h = s.h; r.h_scale = s.h_scale; r.rank = p->rank;
     r.f = p->b; r.f_adapter = p->dim_out * p->rank; r.f_col = p->rank; r.f_rank = 1;
-    return launch_proj_rows(r, st);
+    return launch_proj_adapted(r, s, st);
 }
 
 int64_t vdb_projection_workspace_bytes(const vdb_projection* p, int64_t n, int64_t segments, int backward) {
