@@ -170,7 +170,7 @@ constexpr int pj_tile_bytes(int R) { return R * 128; }
 
 template <int DT, int R> __device__ __forceinline__ int pj_line_swizzle(int k) {
     if constexpr (DT == VDB_F32) return (k >> 2 & 3) << 2;                       // 64-byte spans: the four lane groups read lines k, k + 4, ...
-    else if constexpr (R == 128) return ((k & 3) | (k >> 3 & 1) << 2) << 1;      // 32-byte spans of a 256-byte line
+    else if constexpr (R >= 128) return ((k & 3) | (k >> 3 & 1) << 2) << 1;      // 32-byte spans of a line of 256 or 512 bytes
     else return ((k >> 1 & 1) | (k >> 3 & 1) << 1) << 1;                         // 32-byte spans of a 128-byte line, two lines cover the banks
 }
 
@@ -415,6 +415,84 @@ struct PJProduct {
     }
 };
 
+// ------------------------------------------------------------------------------------------- wide products, 16-bit
+// For the gradient of the matrices, which contracts over rows (both operands lie by k): 256 x 128 per workgroup of four waves,
+// 128 x 64 each, which read three quarters of the LDS bytes per product that 64 x 64 do; 32 rows per stage, a ring of three
+// 24 KiB stages, two workgroups on a CU.  Addresses are 32-bit offsets from bases that move along the rows.
+// (dw of 32 768 rows, 1024 x 768: 88 -> 76 us.  For the rows themselves, whose 64 bytes of k per row are half a cache line, such
+// tiles gained 6 % at 65 536 rows of fp32 output and nothing elsewhere; 256 x 256 tiles of eight waves, half a step apart, 15 % there.)
+constexpr int PJ_WIDE_M = 256, PJ_WIDE_N = 128, PJ_WIDE_S = 3, PJ_WIDE_STAGE = (PJ_WIDE_M + PJ_WIDE_N) * 64;
+constexpr int PJ_WIDE_BYTES = PJ_WIDE_S * PJ_WIDE_STAGE;
+
+// Can the offsets within a stage be 32 bits wide?
+static inline bool pj_offsets_fit(long long rows, long long ld, int esize) { return rows * ld * esize < ((long long)1 << 31); }
+
+// One operand's part of a stage: 32 lines of R columns, piece c of line k in slot c ^ pj_line_swizzle(k).  Columns past the end repeat
+// the last piece of 8: their results are not stored.
+template <int DT, int R> struct PJWideOperand {
+    typedef typename PJ<DT>::T T;
+    static constexpr int P = R / 64, PL = R / 8;
+    const char* base;
+    long long step;
+    unsigned off[P];
+    __device__ __forceinline__ void init(const T* first, long long ld, int cols) {
+        const int last = (cols < R ? cols : R) / 8 - 1;
+        base = (const char*)first;
+        step = 64 * ld;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int p = i * PJ_THREADS + (int)threadIdx.x, k = p / PL, c = p % PL ^ pj_line_swizzle<DT, R>(k);
+            off[i] = (unsigned)k * (unsigned)(ld * 2) + (unsigned)(c < last ? c : last) * 16u;
+        }
+    }
+    // `left` of the 32 lines lie in the operand, the others are zero
+    __device__ __forceinline__ void stage(char* lds, int left) {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const char* src = (i * PJ_THREADS + (int)threadIdx.x) / PL < left ? base + off[i] : (const char*)pj_zero16;
+            __builtin_amdgcn_global_load_lds((const PJ_GLOBAL void*)src, (PJ_LOCAL void*)(lds + (i * PJ_THREADS + wave * 64) * 16), 16, 0, 0);
+        }
+        base += step;
+    }
+};
+
+template <int DT> struct PJWide {
+    static constexpr int BM = 8, BN = 4;
+    PJWideOperand<DT, PJ_WIDE_M> om;
+    PJWideOperand<DT, PJ_WIDE_N> on;
+    long long left;
+    // one load per piece also past the end, so that the waits can count
+    __device__ __forceinline__ void next(char* lds) {
+        const int l = left < 32 ? (left > 0 ? (int)left : 0) : 32;
+        om.stage(lds, l);
+        on.stage(lds + PJ_WIDE_M * 64, l);
+        left -= 32;
+    }
+    __device__ __forceinline__ void run(long long rows, char* lds, int wm, int wn, pj_f32x4 (&acc)[BM][BN]) {
+        left = rows;
+        const int steps = (int)((rows + 31) / 32);
+        if (steps <= 0) return;
+        next(lds);
+        next(lds + PJ_WIDE_STAGE);
+        int cur = 0;
+        for (int t = 0; t < steps; ++t) {
+            pj_wait_and_meet<(PJ_WIDE_S - 2) * 6>();
+            next(lds + (cur == 0 ? 2 : cur - 1) * PJ_WIDE_STAGE);
+            const char* at = lds + cur * PJ_WIDE_STAGE;
+            pj_u32x4 fm[BM], fn[BN];
+            pj_fragments<DT, true, PJ_WIDE_N, BN>(at + PJ_WIDE_M * 64, wn * 64, 0, fn);
+            pj_fragments<DT, true, PJ_WIDE_M, BM>(at, wm * 128, 0, fm);
+#pragma unroll
+            for (int i = 0; i < BM; ++i)
+#pragma unroll
+                for (int j = 0; j < BN; ++j) acc[i][j] = pj_mfma<DT>(fn[j], fm[i], acc[i][j]);
+            cur = cur == 2 ? 0 : cur + 1;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+};
+
 // ------------------------------------------------------------------------------------------- low-rank term
 // The term h f^T of a wave's block, before the main product.  The fp32 intermediate h comes in parts of the rows' type that add up
 // to it (bf16: three; fp16: two, with a power of two for each row that brings its largest entry to 1/2..1, as fp16 could
@@ -622,6 +700,30 @@ struct PJRowsArgs {
     bool vec_out;                // y can be written in aligned pieces of 16 bytes
 };
 
+// Stores a wave's block of 16 B rows by 16 C columns at y as whole cache lines.  A lane holds four columns of a row: stored as they
+// are, a wave's store would be sixteen pieces of 32 or 64 bytes.  Turned in `lds` (BYTES of it, this wave's own) it is four or
+// eight rows of 64 outputs (65 536 x 768 rows out: 112 -> 99 us bf16, 167 -> 157 us fp32), which need not stay in the L2 that the
+// operands of other tiles live in (fp32: 157 -> 142 us).
+template <int ODT, int B, int C, int BYTES>
+__device__ __forceinline__ void pj_store_turned(typename PJ<ODT>::T* y, long long ldy, char* lds, const pj_f32x4 (&acc)[B][C]) {
+    constexpr int LINE = C * 16 * PJ<ODT>::E + 16, LPR = (LINE - 16) / 16, RPI = 64 / LPR;      // lanes to a row, rows to a store
+    constexpr int BI = B * 16 * LINE <= BYTES ? B : B * 8 * LINE <= BYTES ? B / 2 : B / 4;      // blocks of 16 rows that fit
+    static_assert(BI * 16 * LINE <= BYTES, "a wave's part of the ring");
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < B; h += BI) {
+#pragma unroll
+        for (int i = 0; i < BI; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j) pj_store4<ODT>(lds + (i * 16 + li) * LINE + (j * 16 + lh * 4) * PJ<ODT>::E, 0, acc[h + i][j], 4);
+#pragma unroll
+        for (int r = 0; r < BI * 16; r += RPI) {
+            const pj_u32x4 v = *(const pj_u32x4*)(lds + (r + lane / LPR) * LINE + lane % LPR * 16);
+            __builtin_nontemporal_store(v, (pj_u32x4*)((char*)(y + (h * 16 + r + lane / LPR) * ldy) + lane % LPR * 16));
+        }
+    }
+}
+
 // The tile of `tm` rows that this workgroup works on: rows [max(row0, first), min(row0 + tm, row1)); false: none.
 template <bool ADAPT>
 __device__ __forceinline__ bool pj_place(const ProjRows& p, int tm, int col_tiles, int& seg, long long& row0, long long& first,
@@ -665,28 +767,9 @@ proj_rows_kernel(PJRowsArgs a) {
     if constexpr (ADAPT) pj_low_rank<DT, F, B, B>(p, row0 + wm * (R / 2), col0 + wn * (R / 2), am, acc);
     prod.run(pj_lds, wm, wn, acc);
     if (R == 128 && a.vec_out && row0 >= first && row0 + R <= row1 && col0 + R <= p.N) {
-        // A lane holds four columns of a row: stored as they are, a wave's store would be sixteen pieces of 32 or 64 bytes.  Turned
-        // in LDS it is four or eight rows of whole cache lines (65 536 x 768 rows out: 112 -> 99 us bf16, 167 -> 157 us fp32).
-        typedef typename PJ<ODT>::T O;
-        __syncthreads();                                     // the ring is free; from here each wave has a quarter of it
-        constexpr int LINE = (R / 2) * PJ<ODT>::E + 16, LPR = (LINE - 16) / 16, RPI = 64 / LPR;      // lanes to a row, rows to a store
-        constexpr int BI = ODT == VDB_F32 ? B / 2 : B;       // blocks of 16 rows that fit
-        static_assert(BI * 16 * LINE <= PJRing<R>::BYTES / 4, "a wave's part of the ring");
-        char* const mine = pj_lds + wave * (PJRing<R>::BYTES / 4);
-        O* const y = (O*)p.y + (row0 + wm * (R / 2)) * p.ldy + col0 + wn * (R / 2);
-#pragma unroll
-        for (int h = 0; h < B; h += BI) {
-#pragma unroll
-            for (int i = 0; i < BI; ++i)
-#pragma unroll
-                for (int j = 0; j < B; ++j)
-                    pj_store4<ODT>(mine + (i * 16 + li) * LINE + (j * 16 + lh * 4) * PJ<ODT>::E, 0, acc[h + i][j], 4);
-#pragma unroll
-            for (int r = 0; r < BI * 16; r += RPI) {
-                const pj_u32x4 v = *(const pj_u32x4*)(mine + (r + lane / LPR) * LINE + lane % LPR * 16);
-                *(pj_u32x4*)((char*)(y + (h * 16 + r + lane / LPR) * p.ldy) + lane % LPR * 16) = v;
-            }
-        }
+        __syncthreads();                                     // the ring is free: each wave has a quarter of it
+        pj_store_turned<ODT, B, B, PJRing<R>::BYTES / 4>((typename PJ<ODT>::T*)p.y + (row0 + wm * (R / 2)) * p.ldy + col0 + wn * (R / 2), p.ldy,
+                                                         pj_lds + wave * (PJRing<R>::BYTES / 4), acc);
         return;
     }
 #pragma unroll
@@ -766,6 +849,27 @@ struct PJWeightsArgs {
     int m_tiles, n_tiles;
 };
 
+// Segment, output tile and rows [b, e) of this workgroup; item: number of the chunk whose partial sums it leaves, -1: the segment is
+// not split.
+template <bool SPLIT>
+__device__ __forceinline__ bool pj_weights_place(const PJWeightsArgs& a, int& seg, int& tile, long long& b, long long& e, long long& item) {
+    const ProjWeights& p = a.p;
+    item = -1;
+    if constexpr (SPLIT) {
+        if (!pj_find_tile(p.offsets, p.segments, p.n, p.chunk, a.m_tiles * a.n_tiles, blockIdx.x, seg, b, e, tile, item)) return false;
+        if (item >= p.n / p.chunk + p.segments) return false;       // offsets that decrease: more chunks than the workspace holds
+        if (b == pj_clamp(p.offsets[seg], p.n) && e - b <= p.chunk) item = -1;
+        e = e - b < p.chunk ? e : b + p.chunk;
+    } else {
+        seg = blockIdx.x / (a.m_tiles * a.n_tiles);
+        tile = blockIdx.x % (a.m_tiles * a.n_tiles);
+        if (seg >= p.segments) return false;
+        b = pj_clamp(p.offsets[seg], p.n);
+        e = pj_clamp(p.offsets[seg + 1], p.n);
+    }
+    return true;
+}
+
 // dw of one segment, or of one chunk of its rows (SPLIT: a segment of more than one chunk leaves fp32 partial sums, which
 // proj_weights_sum_kernel adds up in the order of the chunks).
 template <int DT, int ODT, bool VEC, bool SPLIT, int R>
@@ -778,19 +882,8 @@ proj_weights_kernel(PJWeightsArgs a) {
     const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     int seg, tile;
-    long long b, e, item = -1;               // rows; number of the chunk, -1: the whole segment
-    if constexpr (SPLIT) {
-        if (!pj_find_tile(p.offsets, p.segments, p.n, p.chunk, a.m_tiles * a.n_tiles, blockIdx.x, seg, b, e, tile, item)) return;
-        if (item >= p.n / p.chunk + p.segments) return;       // offsets that decrease: more chunks than the workspace holds
-        const long long sb = pj_clamp(p.offsets[seg], p.n);
-        if (b == sb && e - b <= p.chunk) item = -1;
-        e = e - b < p.chunk ? e : b + p.chunk;
-    } else {
-        seg = blockIdx.x / (a.m_tiles * a.n_tiles);
-        tile = blockIdx.x % (a.m_tiles * a.n_tiles);
-        b = pj_clamp(p.offsets[seg], p.n);
-        e = pj_clamp(p.offsets[seg + 1], p.n);
-    }
+    long long b, e, item;
+    if (!pj_weights_place<SPLIT>(a, seg, tile, b, e, item)) return;
     const int m0 = tile / a.n_tiles * R, n0 = tile % a.n_tiles * R;
     pj_f32x4 acc[B][B] = {};
     PJProduct<DT, true, true, VEC, R> prod;
@@ -805,6 +898,39 @@ proj_weights_kernel(PJWeightsArgs a) {
 #pragma unroll
         for (int j = 0; j < B; ++j) {
             const int c = n0 + wn * (R / 2) + j * 16 + lh * 4;
+            if (c >= p.N) continue;
+            if (SPLIT && item >= 0) pj_store4<VDB_F32>(p.partial, (item * p.M + m) * p.N + c, acc[i][j], p.N - c);
+            else pj_store4<ODT>(p.dw, ((long long)seg * p.M + m) * p.N + c, acc[i][j], p.N - c);
+        }
+    }
+}
+
+// The same by wide tiles; M and N are multiples of 8.
+template <int DT, int ODT, bool SPLIT>
+__global__ void __launch_bounds__(PJ_THREADS, 2)
+proj_wide_weights_kernel(PJWeightsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char pj_lds[];
+    typedef typename PJ<DT>::T T;
+    constexpr int BM = 8, BN = 4;
+    const ProjWeights& p = a.p;
+    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+    int seg, tile;
+    long long b, e, item;
+    if (!pj_weights_place<SPLIT>(a, seg, tile, b, e, item)) return;
+    const int m0 = tile / a.n_tiles * PJ_WIDE_M, n0 = tile % a.n_tiles * PJ_WIDE_N;
+    pj_f32x4 acc[BM][BN] = {};
+    PJWide<DT> prod;
+    prod.om.init((const T*)p.dy + b * p.lddy + m0, p.lddy, p.M - m0);
+    prod.on.init((const T*)p.x + b * p.ldx + n0, p.ldx, p.N - n0);
+    prod.run(e > b ? e - b : 0, pj_lds, wm, wn, acc);
+#pragma unroll
+    for (int i = 0; i < BM; ++i) {
+        const int m = m0 + wm * 128 + i * 16 + li;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int j = 0; j < BN; ++j) {
+            const int c = n0 + wn * 64 + j * 16 + lh * 4;
             if (c >= p.N) continue;
             if (SPLIT && item >= 0) pj_store4<VDB_F32>(p.partial, (item * p.M + m) * p.N + c, acc[i][j], p.N - c);
             else pj_store4<ODT>(p.dw, ((long long)seg * p.M + m) * p.N + c, acc[i][j], p.N - c);
@@ -922,6 +1048,20 @@ template <int DT, int ODT>
 static hipError_t pj_weights(const ProjWeights& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool vec = pj_aligned(p.dy, p.lddy, E, 16) && pj_aligned(p.x, p.ldx, E, 16) && p.M % V == 0 && p.N % V == 0;
+    if constexpr (DT != VDB_F32)
+        if (vec && p.tile == 128 && pj_offsets_fit(32, p.lddy, 2) && pj_offsets_fit(32, p.ldx, 2)) {
+            PJWeightsArgs a;
+            a.p = p;
+            a.m_tiles = (p.M + PJ_WIDE_M - 1) / PJ_WIDE_M;
+            a.n_tiles = (p.N + PJ_WIDE_N - 1) / PJ_WIDE_N;
+            const long long items = p.chunk > 0 ? p.n / p.chunk + p.segments : p.segments;
+            const dim3 grid((unsigned)((items * a.m_tiles * a.n_tiles + 7) / 8 * 8));
+            auto go = [&](auto kernel) {
+                const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, PJ_WIDE_BYTES);
+                return e == hipSuccess ? pj_launch(kernel, grid, PJ_WIDE_BYTES, a, st) : e;
+            };
+            return p.chunk > 0 ? go(proj_wide_weights_kernel<DT, ODT, true>) : go(proj_wide_weights_kernel<DT, ODT, false>);
+        }
     return vec && p.tile == 128 ? pj_weights_sized<DT, ODT, 128>(p, vec, st) : pj_weights_sized<DT, ODT, 64>(p, vec, st);
 }
 
