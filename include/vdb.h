@@ -259,15 +259,18 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
  * Numerics.  Products are exact and summed in fp32; a result is rounded once, when it is stored.  The low-rank
  * intermediate A x stays in fp32.  NaN and infinities in one row or adapter reach only the rows that use it.
  *
+ * Limits: 2^20 requests, and rows, columns and groups such that no launch needs more than 2^23 workgroups (rows / 64 times the
+ * longer dimension / 64); more is refused with VDB_EINVAL.
+ *
  * Calls enqueue kernels on `stream` and return; they allocate nothing and may be captured into a graph.  `workspace` is device
- * memory of at least vdb_projection_workspace_bytes, aligned to 16 bytes, its contents need not be kept; calls (and
+ * memory of at least vdb_projection_workspace_bytes, aligned to 16 bytes, its contents need not be kept;  calls (and
  * captured graphs) that may run at the same time need workspaces of their own. */
 typedef struct vdb_projection {
     int64_t dim_in, dim_out;     /* 1 .. 65536 */
     int32_t dtype;               /* VDB_F32, VDB_BF16, VDB_F16: type of rows, of incoming gradients and of every weight */
     int32_t out_dtype;           /* type of what a call writes: dtype, or VDB_F32 */
-    int32_t groups;              /* matrices in w; adapted calls take one */
-    int32_t adapters;            /* adapters in a, b, scale; 0: none */
+    int32_t groups;              /* matrices in w, 1 .. 4096; adapted calls take one */
+    int32_t adapters;            /* adapters in a, b, scale, up to 65535; 0: none */
     int32_t rank;                /* of every adapter, 1 .. 128 (smaller ones are filled up with zeros) */
     int32_t reserved;            /* 0 */
     const void*  w;              /* [groups][dim_out][dim_in] */

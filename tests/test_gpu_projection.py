@@ -511,6 +511,71 @@ def test_captured_and_replayed(engine, adapted):
         assert all(torch.equal(a, b) for a, b in zip([dx] + parts, want)), turn
 
 
+def test_large_gradients_captured_and_replayed(engine):
+    """Sizes at which the gradient of the matrices goes through the workspace, captured and replayed beside eager calls."""
+    n = 15000
+    c = Case(n, 768, 640, [0, 4000, 4001, n], "bf16", "f32")
+    dx, dw = (t.clone() for t in c.backward(engine))
+    ws, size = c.ws(engine, True)
+    assert size > 0
+    out = output((n, 768), torch.float32)[1], output(tuple(c.w.shape), torch.float32)[1]
+
+    def step(stream):
+        engine.project_grouped_backward_dev(c.proj, n, c.dy.data_ptr(), 640, c.x.data_ptr(), 768, c.offsets.data_ptr(), out[0].data_ptr(),
+                                            768, out[1].data_ptr(), ws.data_ptr(), size, stream=stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for t in out:
+            t.fill_(SENTINEL)
+        graph.replay()
+        again = c.backward(engine)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], dx) and torch.equal(out[1], dw) and torch.equal(again[1], dw)
+    with pytest.raises(VdbError) as err:
+        engine.project_grouped_backward_dev(c.proj, n, c.dy.data_ptr(), 640, c.x.data_ptr(), 768, c.offsets.data_ptr(), out[0].data_ptr(),
+                                            768, out[1].data_ptr(), ws.data_ptr(), size - 4)
+    assert err.value.code == _lib.EINVAL
+
+
+def test_many_groups(engine):
+    """More groups than rows, and as many as a call takes."""
+    off = [min(3 * max(0, i - 4000), 40) for i in range(4097)]
+    Case(40, 32, 24, off, "bf16", "f32").check(engine)
+    off = [i // 2 for i in range(4097)]
+    Case(2048, 40, 16, off, "f16", "f16").check(engine)
+
+
+def test_calls_from_several_threads(engine):
+    """Calls side by side from host threads, each with its own stream, outputs and workspace."""
+    import threading
+    cases = [Case(200 + 50 * i, 72, 136, [0, 90, 200 + 50 * i], "bf16", "f32", *((3, 16, [2, i % 3]) if i % 2 else ())) for i in range(6)]
+    want = [(c.forward(engine).clone(), [t.clone() for t in c.backward(engine)]) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = [None] * len(cases), []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            for _ in range(10):
+                with torch.cuda.stream(stream):
+                    y = cases[i].forward(engine, stream.cuda_stream)
+                    keep = getattr(cases[i], "keep", None)
+                    got[i] = (y, cases[i].backward(engine, stream.cuda_stream), keep)
+                    stream.synchronize()
+        except Exception as exc:                                  # noqa: BLE001 (reported below)
+            errors.append(exc)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for (y, grads), g in zip(want, got):
+        assert torch.equal(g[0], y) and all(torch.equal(a, b) for a, b in zip(g[1], grads))
+
+
 @pytest.mark.parametrize("metric", [_lib.METRIC_IP, _lib.METRIC_COSINE, _lib.METRIC_L2])
 def test_ingest_and_search_through_projections(engine, table_name, metric):
     """As they are used together: rows of three encoders go through their matrices into one table, queries of several tenants

@@ -60,7 +60,7 @@ ADAPTED = ["adapted", "adapted_backward", "search"]
 
 @pytest.mark.parametrize("fn", GROUPED + ADAPTED)
 @pytest.mark.parametrize("kw", [dict(dim_in=0), dict(dim_in=65537), dict(dim_out=0), dict(dim_out=-1), dict(dtype=3), dict(dtype=-1),
-                                dict(out_dtype=_lib.F16), dict(groups=0), dict(groups=65537), dict(reserved=1), dict(w=None), dict(w=W + 1)])
+                                dict(out_dtype=_lib.F16), dict(groups=0), dict(groups=4097), dict(reserved=1), dict(w=None), dict(w=W + 1)])
 def test_projection_itself_is_checked(fn, kw):
     make = struct if fn in GROUPED else adapter_struct
     assert call(fn, make(**kw)) == _lib.EINVAL
@@ -83,7 +83,7 @@ def test_adapters_are_checked(fn, kw):
     ("grouped_backward", dict(off=None)), ("grouped_backward", dict(lddy=1)), ("grouped_backward", dict(lddx=1)),
     ("grouped_backward", dict(dw=DW + 1)), ("grouped_backward", dict(dx=DY)), ("grouped_backward", dict(dx=X)),
     ("grouped_backward", dict(dw=X)), ("grouped_backward", dict(dw=DY)), ("grouped_backward", dict(dw=W)), ("grouped_backward", dict(dx=DW)),
-    ("adapted", dict(req=-1)), ("adapted", dict(ids=None)), ("adapted", dict(ids=IDS + 2)), ("adapted", dict(ws=None)),
+    ("adapted", dict(req=-1)), ("adapted", dict(req=(1 << 20) + 1)), ("adapted", dict(n=1 << 33)), ("adapted", dict(ids=None)), ("adapted", dict(ids=IDS + 2)), ("adapted", dict(ws=None)),
     ("adapted", dict(wsb=10)), ("adapted", dict(ws=WS + 4)), ("adapted", dict(y=A)), ("adapted", dict(y=B)), ("adapted", dict(y=S)),
     ("adapted", dict(y=IDS)), ("adapted", dict(y=WS)), ("adapted", dict(x=WS)), ("adapted", dict(off=None)), ("adapted", dict(ldx=3)),
     ("adapted_backward", dict(da=None)), ("adapted_backward", dict(db=None)), ("adapted_backward", dict(dx=None, da=None, db=None)),

@@ -550,12 +550,8 @@ proj_weights_sum_kernel(ProjWeights p) {
 }
 
 __global__ void __launch_bounds__(256)
-proj_zero_outside_kernel(float* q, long long dim, long long n, const long long* offsets, int segments) {
-    const long long b = segments > 0 ? pj_clamp(offsets[0], n) : 0, e = segments > 0 ? pj_clamp(offsets[segments], n) : 0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n * dim; i += (long long)gridDim.x * 256) {
-        const long long r = i / dim;
-        if (r < b || r >= e) q[i] = 0.f;
-    }
+proj_zero_kernel(float* q, long long count) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) q[i] = 0.f;
 }
 
 // ------------------------------------------------------------------------------------------- launches
@@ -724,9 +720,9 @@ hipError_t launch_proj_factors(const ProjFactor& p, const ProjFactor& b, hipStre
     PJ_TYPES(p.dtype, p.out_dtype, PJ_BY_RANK(return (factor_typed<DT, ODT, NRB>(p, b, st))));
 }
 
-hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st) {
-    const long long blocks = (n * dim + 255) / 256;
-    hipLaunchKernelGGL(proj_zero_outside_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, q, dim, n, offsets, segments);
+hipError_t launch_proj_zero(float* q, long long count, hipStream_t st) {
+    const long long blocks = (count + 255) / 256;
+    hipLaunchKernelGGL(proj_zero_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, q, count);
     return hipGetLastError();
 }
 

@@ -99,7 +99,6 @@ hipError_t launch_proj_adapted(const ProjRows& p, const ProjShrink& s, hipStream
 // both intermediates of a backward pass, of dy and of x; the gradients of both factors
 hipError_t launch_proj_shrink_pair(const ProjShrink& g, const ProjShrink& h, hipStream_t st);
 hipError_t launch_proj_factors(const ProjFactor& a, const ProjFactor& b, hipStream_t st);
-// rows [n, dim] of q outside every segment become zero
-hipError_t launch_proj_zero_outside(float* q, long long dim, long long n, const long long* offsets, int segments, hipStream_t st);
+hipError_t launch_proj_zero(float* q, long long count, hipStream_t st);
 
 }  // namespace vdb

@@ -949,6 +949,9 @@ static hipError_t pj_launch(K kernel, dim3 grid, size_t lds, const A& args, hipS
     return hipGetLastError();
 }
 
+// Segments that can have rows: each adds at most one tile to those that the rows alone would fill.
+static inline long long pj_filled(long long n, int segments) { return n < segments ? n : segments; }
+
 // 64 x 64 tiles where 128 x 128 ones would leave CUs without work (bf16, 768 x 768, 8 groups: 8192 rows, 408 tiles of 128 x 128, 18 us
 // and 30 by 64 x 64).
 static inline bool pj_small_tiles(long long tiles128) { return tiles128 < 256; }
@@ -967,7 +970,7 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     a.col_tiles = (p.N + R - 1) / R;
     constexpr int E = PJ<DT>::E, V = 16 / E;
     a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 16);
-    const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + p.segments;
+    const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + pj_filled(p.n, p.segments);
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
     const bool fv = pj_factor_vec<DT, V>(p);
@@ -996,7 +999,7 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
     a.col_tiles = (p.N + 15) / 16;
     constexpr int V = 16 / PJ<DT>::E;
     a.vec_out = false;
-    const long long row_tiles = p.row_adapter ? (p.n + 15) / 16 : p.n / 16 + p.segments;
+    const long long row_tiles = p.row_adapter ? (p.n + 15) / 16 : p.n / 16 + pj_filled(p.n, p.segments);
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const bool fv = pj_factor_vec<DT, V>(p);
 #define PJ_FEW(NK, VEC)                                                                          \
@@ -1034,7 +1037,7 @@ static hipError_t pj_weights_sized(const ProjWeights& p, bool vec, hipStream_t s
     const dim3 grid((unsigned)((long long)p.segments * a.m_tiles * a.n_tiles));
     const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
     if (p.chunk > 0) {
-        const dim3 chunks((unsigned)(((p.n / p.chunk + p.segments) * a.m_tiles * a.n_tiles + 7) / 8 * 8));
+        const dim3 chunks((unsigned)(((p.n / p.chunk + pj_filled(p.n, p.segments)) * a.m_tiles * a.n_tiles + 7) / 8 * 8));
         if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st);
         else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st)
                         : pj_launch(proj_weights_kernel<DT, ODT, false, true, R>, chunks, lds, a, st);
@@ -1054,7 +1057,7 @@ static hipError_t pj_weights(const ProjWeights& p, hipStream_t st) {
             a.p = p;
             a.m_tiles = (p.M + PJ_WIDE_M - 1) / PJ_WIDE_M;
             a.n_tiles = (p.N + PJ_WIDE_N - 1) / PJ_WIDE_N;
-            const long long items = p.chunk > 0 ? p.n / p.chunk + p.segments : p.segments;
+            const long long items = p.chunk > 0 ? p.n / p.chunk + pj_filled(p.n, p.segments) : p.segments;
             const dim3 grid((unsigned)((items * a.m_tiles * a.n_tiles + 7) / 8 * 8));
             auto go = [&](auto kernel) {
                 const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, PJ_WIDE_BYTES);

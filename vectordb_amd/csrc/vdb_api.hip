@@ -2027,7 +2027,7 @@ static int proj_check(const vdb_projection* p, int64_t n, int64_t segments, bool
     if (p->dtype != VDB_F32 && p->dtype != VDB_BF16 && p->dtype != VDB_F16) return fail(VDB_EINVAL, "unknown projection dtype");
     if (p->out_dtype != p->dtype && p->out_dtype != VDB_F32) return fail(VDB_EINVAL, "out_dtype must be dtype or VDB_F32");
     if (p->reserved != 0) return fail(VDB_EINVAL, "the reserved field of a projection must be 0");
-    if (p->groups < 1 || p->groups > 65536) return fail(VDB_EINVAL, "groups must be in [1, 65536]");
+    if (p->groups < 1 || p->groups > 4096) return fail(VDB_EINVAL, "groups must be in [1, 4096]");
     if (n < 0 || segments < 0) return fail(VDB_EINVAL, "negative number of rows or segments");
     const uintptr_t e = p->dtype == VDB_F32 ? 4 : 2;
     if (!p->w || (uintptr_t)p->w % e) return fail(VDB_EINVAL, "w is null or not aligned to its type");
@@ -2037,10 +2037,10 @@ static int proj_check(const vdb_projection* p, int64_t n, int64_t segments, bool
         if (p->rank < 1 || p->rank > PROJ_MAX_RANK) return fail(VDB_EINVAL, "rank must be in [1, 128]");
         if (!p->a || !p->b || (uintptr_t)p->a % e || (uintptr_t)p->b % e) return fail(VDB_EINVAL, "a or b is null or not aligned to its type");
         if ((uintptr_t)p->scale % 4) return fail(VDB_EINVAL, "scale is not aligned to its type");
-        if (segments > (1 << 24)) return fail(VDB_EINVAL, "more than 2^24 requests");
+        if (segments > (1 << 20)) return fail(VDB_EINVAL, "more than 2^20 requests");
     }
     // every launch stays within 2^23 workgroups
-    const int64_t lim = (int64_t)1 << 23, td = 128;
+    const int64_t lim = (int64_t)1 << 23, td = 64;
     const int64_t ct = (std::max(p->dim_in, p->dim_out) + td - 1) / td;
     if (n > (lim - 8) / ct * 16 || (n / td + (adapted ? 1 : p->groups) + 1) * ct > lim - 8 ||
         (int64_t)p->groups * ((p->dim_in + td - 1) / td) * ((p->dim_out + td - 1) / td) > lim)
@@ -2378,7 +2378,7 @@ int vdb_search_projected_dev(const char* name, const vdb_projection* p, int64_t 
         rc = ensure(ws->proj, hb + qb, ws->last_stream);
         if (rc == VDB_OK) {
             float* const q = (float*)((char*)ws->proj.p + hb);
-            hipError_t e = launch_proj_zero_outside(q, t->dim, nq, (const long long*)offsets, (int)requests, st);
+            hipError_t e = launch_proj_zero(q, nq * t->dim, st);        // queries outside every request are zero vectors
             if (e == hipSuccess && requests > 0)
                 e = proj_adapted(p, nq, x, ldx, offsets, adapter_ids, requests, q, t->dim, VDB_F32, ws->proj.p, st);
             if (e != hipSuccess) rc = fail(VDB_EHIP, std::string("projection: ") + hipGetErrorString(e));
