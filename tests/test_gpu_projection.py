@@ -646,3 +646,40 @@ def test_projected_insert_and_search_refusals(engine, table_name):
     insert([0, 5, 20])
     insert([0, 0, 20])
     assert engine.count(table_name) == 40
+
+
+# middle sizes in fp32: 32 x 32 tiles, aligned and not, one adapter, a few and many in 16 rows
+MIDDLE = [
+    (1100, 384, 384, 0),
+    (700, 515, 515, 0),
+    (1090, 384, 372, 8),
+    (610, 640, 640, 64),
+    (690, 261, 515, 19),
+]
+
+
+@pytest.mark.parametrize("n,din,dout,rank", MIDDLE)
+def test_middle_sizes(engine, n, din, dout, rank):
+    if not rank:
+        Case(n, din, dout, [1, 300, 300, 301, 640, n - 3], "f32", "f32").check(engine)
+        return
+    off = list(range(0, 40)) + [56, 60, 64, 300, 301, n - 3]
+    ids = [(5 * i) % 12 - 1 for i in range(len(off) - 1)]
+    Case(n, din, dout, off, "f32", "f32", 11, rank, ids).check(engine)
+    Case(n, din, dout, [0, n], "f32", "f32", 2, rank, [1]).check(engine)
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,rank,segments", [(1, 8, 8, 1, 1), (70, 33, 17, 5, 9), (300, 384, 384, 8, 200), (5000, 136, 200, 64, 3),
+                                                      (9000, 256, 264, 0, 5), (40, 16, 24, 0, 3)])
+def test_workspace_of_the_stated_size_is_not_exceeded(engine, n, din, dout, rank, segments, dtype, out):
+    off = [n * s // segments for s in range(segments + 1)]
+    ids = [s % 3 - 1 for s in range(segments)] if rank else None
+    case = Case(n, din, dout, off, dtype, out, 2 if rank else 0, rank, ids)
+    for call, backward in ((case.forward, False), (case.backward, True)):
+        case.keep = None
+        call(engine)
+        torch.cuda.synchronize()
+        size = engine.projection_workspace_bytes(case.proj, n, segments, backward)
+        if case.keep is not None:
+            assert bool(case.keep.view(torch.uint8)[size:].view(torch.float32).isnan().all())

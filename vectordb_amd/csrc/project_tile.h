@@ -161,7 +161,7 @@ __device__ __forceinline__ void pj_each_request(const long long* offsets, const 
 }
 
 // ------------------------------------------------------------------------------------------- tiles in LDS
-// One operand tile: R = 64 or 128 rows (or columns) of the product by 128 bytes of the contracted axis, kept as it lies in
+// One operand tile: R = 32, 64 or 128 rows (or columns) of the product by 128 bytes of the contracted axis, kept as it lies in
 // memory in 16-byte pieces whose place is swizzled so that the fragment reads below touch every bank once:
 //   contiguous along k (BYK = false): row r is 128 bytes, piece c sits in slot c ^ ((r >> 1) & 7)
 //   contiguous along the rows (BYK = true): one line per k, piece c of line k in slot c ^ pj_line_swizzle(k)
@@ -169,7 +169,7 @@ constexpr int PJ_THREADS = 256;
 constexpr int pj_tile_bytes(int R) { return R * 128; }
 
 template <int DT, int R> __device__ __forceinline__ int pj_line_swizzle(int k) {
-    if constexpr (DT == VDB_F32) return (k >> 2 & 3) << 2;                       // 64-byte spans: the four lane groups read lines k, k + 4, ...
+    if constexpr (DT == VDB_F32) return (k >> 2 & (R == 32 ? 1 : 3)) << 2;       // 64-byte spans: the four lane groups read lines k, k + 4, ...
     else if constexpr (R >= 128) return ((k & 3) | (k >> 3 & 1) << 2) << 1;      // 32-byte spans of a line of 256 or 512 bytes
     else return ((k >> 1 & 1) | (k >> 3 & 1) << 1) << 1;                         // 32-byte spans of a 128-byte line, two lines cover the banks
 }
@@ -244,7 +244,7 @@ __device__ __forceinline__ void pj_fragments(const char* lds, int row, int kk, p
     } else if constexpr (DT == VDB_F32) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            const int c = ((row + i * 16 + li) >> 2) ^ (lh << 2);
+            const int c = ((row + i * 16 + li) >> 2) ^ pj_line_swizzle<DT, R>(lh * 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 f[i][j] = *(const unsigned*)(lds + (kk * 16 + lh * 4 + j) * LINE + (c << 4) + (li & 3) * 4);
@@ -327,9 +327,10 @@ template <int N> __device__ __forceinline__ void pj_wait_and_meet() {
 }
 
 // Tiles of a launch: 64 x 64 with four stages of k in flight where there are few of them, 128 x 128 with two stages and
-// two workgroups on a CU where there are many (see pj_small_tiles).
+// two workgroups on a CU where there are many (see pj_small_tiles); fp32, whose products take eight times as long, 32 x 32
+// with eight stages where 64 x 64 leave CUs without work.
 template <int R> struct PJRing {
-    static constexpr int STAGES = R == 64 ? 4 : 2;
+    static constexpr int STAGES = R == 32 ? 8 : R == 64 ? 4 : 2;
     static constexpr int BYTES = STAGES * 2 * pj_tile_bytes(R);
     static constexpr int HALVES = 2 * 2 * pj_tile_bytes(R);          // through registers: two stages
 };
@@ -508,6 +509,10 @@ template <int DT> struct PJWide {
 //   PJ_F_ANY     neither
 enum { PJ_F_ANY = 0, PJ_F_RANKS = 1, PJ_F_COLS = 2 };
 
+// Waits until the matrix unit has written t: the compiler's own wait for an fp32 product (10 states) was seen to fall away where the
+// products end a loop whose exit reads them at once (columns 3 mod 4 of a 32 x 32 tile held the sum without its last step).
+__device__ __forceinline__ void pj_settle(pj_f32x4& t) { asm volatile("s_nop 15" : "+v"(t)); }
+
 // 16 rows by one adapter on the matrix unit; t: lane's row by columns colb + 16 j + 4 (l / 16) + 0..3
 template <int DT, int F, int C>
 __device__ __forceinline__ void pj_low_rank_block(const ProjRows& p, long long mc, int colb, int a, pj_f32x4 (&t)[C]) {
@@ -537,6 +542,9 @@ __device__ __forceinline__ void pj_low_rank_block(const ProjRows& p, long long m
             if constexpr (F != PJ_F_RANKS) asm volatile("" ::: "memory");       // one block's loads at a time: registers
         }
     }
+    if constexpr (DT == VDB_F32)
+#pragma unroll
+        for (int j = 0; j < C; ++j) pj_settle(t[j]);
 }
 
 // All B blocks of 16 rows by one adapter.
@@ -1016,6 +1024,11 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
 // and 13.1).
 constexpr long long PJ_FEW_TILES = 64;
 
+// fp32 takes 32 x 32 tiles where 64 x 64 would leave half of the CUs without one (384 x 384, in a graph: 1024 rows, 99 tiles, 10.0 us
+// by 32 x 32 and 13.1 by 64 x 64; 1000 rows of 515 x 387, 126 tiles, 15.0 and 23.4; 2048 rows, 195 tiles, 18.4 and 13.6; 1024 x 768,
+// 192 tiles, 30.4 and 28.1).
+constexpr long long PJ_F32_TILES = 128;
+
 template <int DT, int ODT>
 static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
     constexpr int E = PJ<DT>::E, V = 16 / E;
@@ -1024,6 +1037,8 @@ static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
     const long long tiles = ((p.n + 127) / 128 + (p.row_adapter ? 0 : p.segments / 2)) * ((p.N + 127) / 128);
     const long long tiles64 = ((p.n + 63) / 64) * ((p.N + 63) / 64);
     if (tiles64 <= PJ_FEW_TILES) return pj_few<DT, ODT>(p, vec, st);
+    if constexpr (DT == VDB_F32)
+        if (((p.n + 63) / 64 + (p.row_adapter ? 0 : p.segments / 2)) * ((p.N + 63) / 64) < PJ_F32_TILES) return pj_rows_sized<DT, ODT, 32>(p, vec, st);
     const bool big = vec && !pj_small_tiles(tiles) && (!p.row_adapter || pj_factor_vec<DT, V>(p));
     return big ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
 }
