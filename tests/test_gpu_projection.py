@@ -683,3 +683,41 @@ def test_workspace_of_the_stated_size_is_not_exceeded(engine, n, din, dout, rank
         size = engine.projection_workspace_bytes(case.proj, n, segments, backward)
         if case.keep is not None:
             assert bool(case.keep.view(torch.uint8)[size:].view(torch.float32).isnan().all())
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,adapters,rank", [(2100, 72, 136, 1, 5), (5000, 64, 200, 3, 20), (9000, 136, 72, 2, 70), (12000, 40, 66, 17, 8)])
+def test_factor_gradients_of_many_rows_to_an_adapter(engine, n, din, dout, adapters, rank, dtype, out):
+    """Rows of an adapter shared by several workgroups, requests that end inside blocks of 16 rows, one adapter without rows."""
+    cuts = [0, n // 3 + 1, n // 3 + 1, n // 2, n // 2 + 5, n - 7]
+    ids = [0, 1 % adapters, 0, adapters - 1, 0]
+    case = Case(n, din, dout, cuts, dtype, out, adapters, rank, ids)
+    case.check(engine)
+    first = [t.clone() for t in case.backward(engine)[1:]]
+    again = case.backward(engine)[1:]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,rank", [(4100, 256, 384, 16), (33000, 256, 520, 9)])
+def test_requests_that_meet_in_a_tile(engine, n, din, dout, rank, dtype, out):
+    """Requests of 5 to 40 rows and of hundreds: one, a few and many adapters in the rows of a wave, some without one; what an
+    adapter of infinities holds stays with its own rows."""
+    off, i = [0], 0
+    while off[-1] < n - 50:
+        off.append(min(off[-1] + (5, 40, 17, 700, 33, 24, 150)[i % 7], n - 50))
+        i += 1
+    ids = [(3 * s) % 8 - 1 for s in range(len(off) - 1)]
+    case = Case(n, din, dout, off, dtype, out, 7, rank, ids)
+    case.check(engine)
+    clean = case.forward(engine).clone()
+    case.b[4].fill_(float("inf"))
+    got = case.forward(engine)
+    torch.cuda.synchronize()
+    other = torch.ones(n, dtype=torch.bool)
+    for s, b, e in spans(off, n):
+        if ids[s] == 4:
+            other[b:e] = False
+    assert torch.equal(got.cpu()[other], clean.cpu()[other])
+    assert not torch.isfinite(got.cpu()[~other].float()).all(dim=1).any()

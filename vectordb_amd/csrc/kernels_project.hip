@@ -42,7 +42,7 @@ __device__ __forceinline__ void pj_shrink_load_x(const ProjShrink& p, const type
 #pragma unroll
     for (int u = 0; u < XS; ++u) {
         const int k = k0 + u * stride + lh * V;
-        if constexpr (XV) xa[u] = *(const pj_u32x4*)(k < p.K ? x + k : (const T*)pj_zero16);
+        if constexpr (XV) xa[u] = pj_load_if<pj_u32x4>(k < p.K, x + k);
         else xa[u] = pj_piece<T>(x + k, p.K - k);
     }
 }
@@ -69,14 +69,14 @@ __device__ __forceinline__ void pj_shrink_steps(const ProjShrink& p, const pj_u3
             for (int i = 0; i < NRB; ++i) {
                 const int c = i * 64 + lane;
                 const bool in = c < 32 * ppl && kb + c / ppl < p.K;
-                fa[u][i].v = *(const pj_u32x4*)(in ? f + (unsigned)kb * fk + (unsigned)c * 8u : (const T*)pj_zero16);
+                fa[u][i].v = pj_load_if<pj_u32x4>(in, f + (unsigned)kb * fk + (unsigned)c * 8u);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NRB; ++i) {
                 const int q = i * 16 + li;
                 const unsigned at = (unsigned)q * fr + (unsigned)k * fk;
-                if constexpr (F == PJ_S_FK) fa[u][i].v = *(const pj_u32x4*)(k < p.K && q < p.rank ? f + at : (const T*)pj_zero16);
+                if constexpr (F == PJ_S_FK) fa[u][i].v = pj_load_if<pj_u32x4>(k < p.K && q < p.rank, f + at);
                 else
 #pragma unroll
                     for (int j = 0; j < V; ++j) fa[u][i].t[j] = k + j < p.K && q < p.rank ? f[at + (unsigned)j * fk] : (T)0;
@@ -338,7 +338,7 @@ proj_adapt_few_kernel(ProjRows p, ProjShrink s, int col_tiles) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         const int col = c0 + lh * 4 + n;
-        fv[n].v = *(const pj_u32x4*)(some ? f + (unsigned)(col < p.N ? col : p.N - 1) * (unsigned)p.f_col + (unsigned)q : (const T*)pj_zero16);
+        fv[n].v = pj_load_if<pj_u32x4>(some, f + (unsigned)(col < p.N ? col : p.N - 1) * (unsigned)p.f_col + (unsigned)q);
     }
     const float sc = some ? (s.scale ? s.scale[am[0]] : 1.f) : 0.f;
     // the adapters of the 16 rows one after the other, the factor of the next one on its way while one is multiplied
@@ -350,7 +350,7 @@ proj_adapt_few_kernel(ProjRows p, ProjShrink s, int col_tiles) {
             const int k = wave * KS + u * 4 * KS + lh * V;
 #pragma unroll
             for (int i = 0; i < NRB; ++i)
-                fa[u][i] = *(const pj_u32x4*)(k < s.K && i * 16 + li < s.rank ? a + (unsigned)(i * 16 + li) * (unsigned)s.f_rank + (unsigned)k : (const T*)pj_zero16);
+                fa[u][i] = pj_load_if<pj_u32x4>(k < s.K && i * 16 + li < s.rank, a + (unsigned)(i * 16 + li) * (unsigned)s.f_rank + (unsigned)k);
         }
     };
     pj_u32x4 fa[XS][NRB], fb[XS][NRB];
@@ -410,30 +410,44 @@ proj_adapt_few_kernel(ProjRows p, ProjShrink s, int col_tiles) {
 }
 
 // ------------------------------------------------------------------------------------------- gradient of the factors
-// One adapter's [rank] x 64 columns: the eight waves take its rows 16 at a time in turn, over every request that names the
-// adapter, and add up in wave order.  Products on the fp32 matrix unit: h is fp32, x is widened.
+// One adapter's [rank] x 64 columns: eight waves, of one workgroup or of several, take its rows 16 at a time in turn, over every
+// request that names the adapter, and add up in wave order.  Several workgroups leave their sums in `partial`, and
+// proj_factor_sum_kernel adds them up in their order.  Products on the fp32 matrix unit: h is fp32, x is widened.
 // Lane l loads columns 4 (l % 16) + 0..3 of a row, so that product j of a step holds columns j, 4 + j, 8 + j, ...
-// The rows of the next turn are loaded while the current ones are multiplied.
+// The rows of the next turns are loaded while the current ones are multiplied.
 constexpr int PJ_FACTOR_WAVES = 8;
 
 template <int DT, int NRB, bool XV> struct PJFactorRows {
     typedef typename PJ<DT>::T T;
-    typedef T tx4 __attribute__((ext_vector_type(4)));
-    tx4 x[4];
-    float h[4][NRB];
+    union { T t[4]; unsigned u[PJ<DT>::E]; } x[4];
+    union { float f; unsigned u; } h[4][NRB];
+    // Rows behind the request's last are read as that one and masked, so that no load waits for a branch; columns and ranks outside
+    // are read as the first ones, and what comes of them is not stored.
     __device__ __forceinline__ void load(const ProjFactor& p, long long r, long long e, int c0) {
         const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const long long i = r + u * 4 + lh;
-            const bool ok = i < e;
-            const T* px = (const T*)p.x + (ok ? i : 0) * p.ldx + c0;
-            if constexpr (XV) x[u] = *(const tx4*)(ok && c0 < p.N ? px : (const T*)pj_zero16);
+            const long long i = r + u * 4 + lh, k = i < e ? i : e - 1;
+            const T* px = (const T*)p.x + k * p.ldx;
+            if constexpr (XV) __builtin_memcpy(x[u].t, __builtin_assume_aligned(px + (c0 < p.N ? c0 : 0), 4 * sizeof(T)), 4 * sizeof(T));
             else
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[u][j] = ok && c0 + j < p.N ? px[j] : (T)0;
+                for (int j = 0; j < 4; ++j) x[u].t[j] = px[c0 + j < p.N ? c0 + j : 0];
 #pragma unroll
-            for (int q = 0; q < NRB; ++q) h[u][q] = ok && q * 16 < p.rp ? p.h[i * p.rp + q * 16 + li] : 0.f;
+            for (int q = 0; q < NRB; ++q) h[u][q].f = p.h[k * p.rp + (q * 16 < p.rp ? q * 16 : 0) + li];
+        }
+    }
+    __device__ __forceinline__ void mask(long long r, long long e) {
+        const int lh = (threadIdx.x & 63) >> 4;
+        if (r + 16 <= e) return;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            unsigned ok = r + u * 4 + lh < e ? ~0u : 0u;
+            asm volatile("" : "+v"(ok));                     // not a branch around the loads
+#pragma unroll
+            for (int j = 0; j < PJ<DT>::E; ++j) x[u].u[j] &= ok;
+#pragma unroll
+            for (int q = 0; q < NRB; ++q) h[u][q].u &= ok;
         }
     }
     __device__ __forceinline__ void multiply(pj_f32x4 (&acc)[NRB][4]) const {
@@ -443,46 +457,85 @@ template <int DT, int NRB, bool XV> struct PJFactorRows {
             for (int q = 0; q < NRB; ++q)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[q][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(pj_to_f32<DT>(x[u][j]), h[u][q], acc[q][j], 0, 0, 0);
+                    acc[q][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(pj_to_f32<DT>(x[u].t[j]), h[u][q].f, acc[q][j], 0, 0, 0);
     }
 };
 
-// blockIdx.z: the gradient of A, of B.
+// Where workgroup `split` of an adapter leaves its sum of 64 columns: NRB blocks of 16 ranks, 4 products, 64 lanes of 4 values.
+template <int NRB> __device__ __forceinline__ pj_f32x4* pj_factor_partial(const ProjFactor& p, int split, int adapter, int block) {
+    return (pj_f32x4*)p.partial + (((long long)split * p.adapters + adapter) * ((p.N + 63) / 64) + block) * (NRB * 4 * 64);
+}
+
+// One block of 16 ranks by columns lh * 16 + 4 u + j of the block at n0, product j, into the gradient.
+template <int ODT> __device__ __forceinline__ void pj_factor_store(const ProjFactor& p, int adapter, int k, int n0, int j, const pj_f32x4& v) {
+    const int lh = (threadIdx.x & 63) >> 4;
+    if (k >= p.rank) return;
+    typename PJ<ODT>::T* out = (typename PJ<ODT>::T*)p.out + (long long)adapter * p.rank * p.N;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int c = n0 + lh * 16 + u * 4 + j;
+        if (c < p.N) out[p.by_col ? (long long)c * p.rank + k : (long long)k * p.N + c] = pj_from_f32<ODT>(v[u]);
+    }
+}
+
+// blockIdx.z: the gradient of A, of B, for each of the splits.
 template <int DT, int ODT, int NRB, bool XV>
 __global__ void __launch_bounds__(PJ_FACTOR_WAVES * 64)
 proj_factor_kernel(ProjFactor pa, ProjFactor pb) {
-    const ProjFactor& p = blockIdx.z == 0 ? pa : pb;
+    const ProjFactor& p = blockIdx.z % 2 == 0 ? pa : pb;
     if ((int)blockIdx.x * 64 >= p.N) return;
-    typedef typename PJ<ODT>::T O;
-    constexpr int W = PJ_FACTOR_WAVES;
+    constexpr int W = PJ_FACTOR_WAVES, D = NRB <= 2 ? 4 : 2;           // blocks of rows in registers
     __shared__ pj_f32x4 part[W - 1][4][64];
-    const int lane = threadIdx.x & 63, li = lane & 15, lh = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, li = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.z / 2, all = W * p.splits, mine = split * W + wave;
     const int n0 = blockIdx.x * 64, ad = blockIdx.y, c0 = n0 + li * 4;
     pj_f32x4 acc[NRB][4] = {};
-    PJFactorRows<DT, NRB, XV> rows[2];
-    int turn = 0;                          // blocks of 16 rows met so far
-    bool held = false;                     // rows[0] holds a block that has not been multiplied
-    for (int s0 = 0; s0 < p.segments; s0 += 64) {
-        const bool hit = s0 + lane < p.segments && p.ids[s0 + lane] == ad;
-        unsigned long long mask = __ballot(hit);
-        while (mask) {
+    // this wave's blocks of 16 rows, one after the other: rows [r, min(r + 16, e))
+    int s0 = -64, turn = 0;                // requests looked at; blocks of the adapter met so far, modulo all
+    unsigned long long mask = 0;           // requests of the 64 at s0 that are left
+    long long r = 0, e = 0;
+    auto next = [&]() {
+        r += all * 16;
+        while (r >= e) {
+            while (!mask) {
+                s0 += 64;
+                if (s0 >= p.segments) return false;
+                mask = __ballot(s0 + lane < p.segments && p.ids[s0 + lane] == ad);
+            }
             const int s = s0 + __builtin_ctzll(mask);
             mask &= mask - 1;
-            const long long b = pj_clamp(p.offsets[s], p.n), e = pj_clamp(p.offsets[s + 1], p.n);
-            if (e <= b) continue;
-            const long long blocks = (e - b + 15) / 16;
-            const int start = (wave - turn % W + W) % W;         // this wave's first block of the request
-            turn = (int)((turn + blocks) % W);
-            for (long long i = start; i < blocks; i += W) {
-                rows[1].load(p, b + i * 16, e, c0);
-                if (held) rows[0].multiply(acc);
-                rows[0] = rows[1];
-                held = true;
-            }
+            const long long b = pj_clamp(p.offsets[s], p.n);
+            e = pj_clamp(p.offsets[s + 1], p.n);
+            if (e <= b) { r = e; continue; }
+            r = b + (long long)((mine - turn + all) % all) * 16;
+            turn = (int)((turn + (e - b + 15) / 16) % all);
+        }
+        return true;
+    };
+    PJFactorRows<DT, NRB, XV> rows[D];
+    long long at[D], end[D];               // the slots' rows; at == end: empty
+#pragma unroll
+    for (int u = 0; u < D; ++u) at[u] = end[u] = 0;
+    bool more = true;
+    auto fill = [&](int u) {
+        more = more && next();
+        at[u] = end[u] = 0;
+        if (!more) return;
+        at[u] = r; end[u] = e;
+        rows[u].load(p, r, e, c0);
+    };
+#pragma unroll
+    for (int u = 0; u < D - 1; ++u) fill(u);
+    for (bool any = true; any;) {
+#pragma unroll
+        for (int u = 0; u < D; ++u) {
+            fill((u + D - 1) % D);
+            any = at[u] < end[u];
+            if (!any) break;
+            rows[u].mask(at[u], end[u]);
+            rows[u].multiply(acc);
         }
     }
-    if (held) rows[0].multiply(acc);
-    O* out = (O*)p.out + (long long)ad * p.rank * p.N;
 #pragma unroll
     for (int q = 0; q < NRB; ++q) {
         __syncthreads();
@@ -490,20 +543,29 @@ proj_factor_kernel(ProjFactor pa, ProjFactor pb) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) part[wave - 1][j][lane] = acc[q][j];
         __syncthreads();
-        const int k = q * 16 + li;
-        if (wave || k >= p.rank) continue;
+        if (wave) continue;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int j = 0; j < 4; ++j) {
+            pj_f32x4 v = acc[q][j];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = n0 + lh * 16 + u * 4 + j;
-                if (c >= p.N) continue;
-                float v = acc[q][j][u];
-#pragma unroll
-                for (int w = 0; w < W - 1; ++w) v += part[w][j][lane][u];
-                out[p.by_col ? (long long)c * p.rank + k : (long long)k * p.N + c] = pj_from_f32<ODT>(v);
-            }
+            for (int w = 0; w < W - 1; ++w) v += part[w][j][lane];
+            if (p.splits > 1) pj_factor_partial<NRB>(p, split, ad, blockIdx.x)[(q * 4 + j) * 64 + lane] = v;
+            else pj_factor_store<ODT>(p, ad, q * 16 + li, n0, j, v);
+        }
     }
+}
+
+// The sum of an adapter's partial sums; blockIdx.z as above, one block of 16 ranks for each further z.
+template <int ODT, int NRB>
+__global__ void __launch_bounds__(256)
+proj_factor_sum_kernel(ProjFactor pa, ProjFactor pb) {
+    const ProjFactor& p = blockIdx.z % 2 == 0 ? pa : pb;
+    if ((int)blockIdx.x * 64 >= p.N) return;
+    const int lane = threadIdx.x & 63, j = threadIdx.x >> 6, q = blockIdx.z / 2, ad = blockIdx.y;
+    pj_f32x4 v = {};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) v += pj_factor_partial<NRB>(p, s, ad, blockIdx.x)[(q * 4 + j) * 64 + lane];
+    pj_factor_store<ODT>(p, ad, q * 16 + (lane & 15), blockIdx.x * 64, j, v);
 }
 
 // dw of the segments that were split, and zeros for those without rows: the chunks' partial sums in their order.
@@ -642,11 +704,16 @@ static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
 template <int DT, int ODT, int NRB>
 static hipError_t factor_typed(const ProjFactor& p, const ProjFactor& b, hipStream_t st) {
     const int most = p.N > b.N ? p.N : b.N;
-    const dim3 grid((unsigned)((most + 63) / 64), (unsigned)p.adapters, 2), threads(PJ_FACTOR_WAVES * 64);
+    const dim3 grid((unsigned)((most + 63) / 64), (unsigned)p.adapters, 2 * p.splits), threads(PJ_FACTOR_WAVES * 64);
     const bool xv = pj_aligned(p.x, p.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && p.N % 4 == 0 &&
                     pj_aligned(b.x, b.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && b.N % 4 == 0;
     if (xv) hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, true>), grid, threads, 0, st, p, b);
     else hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, false>), grid, threads, 0, st, p, b);
+    if (p.splits > 1) {
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((proj_factor_sum_kernel<ODT, NRB>), dim3(grid.x, grid.y, 2 * ((p.rank + 15) / 16)), dim3(256), 0, st, p, b);
+    }
     return hipGetLastError();
 }
 

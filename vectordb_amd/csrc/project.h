@@ -75,11 +75,28 @@ inline void proj_weights_plan(long long n, int segments, int M, int N, int& tile
     if (c < n) chunk = (int)c;
 }
 
+// Workgroups that share the rows of an adapter, as many as leave 512 rows to each, and 16 over all adapters: with few adapters
+// there are too few workgroups, with many the ones that find no rows cost more than the others gain (whole backward pass, 768 x
+// 768 bf16, rank 16, alone and shared: 16 384 rows of 1 adapter 174 and 76 us, of 4 adapters 105 and 78, of 24 adapters by two 80
+// and 83; 1024 x 768 fp16, rank 64, 4096 rows of 10 adapters by three 74 and 81).
+constexpr int PJ_FACTOR_SHARES = 16;
+inline int proj_factor_splits(long long n, int adapters) {
+    const long long most = n / 512, want = PJ_FACTOR_SHARES / adapters;
+    const long long s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : s);
+}
+// floats of the partial sums of one factor's gradient
+inline long long proj_factor_partial(int splits, int adapters, int rank, long long N) {
+    const int nrb = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
+    return splits > 1 ? (long long)splits * adapters * ((N + 63) / 64) * (nrb * 1024) : 0;
+}
+
 // out[a][q][c] (or, by_col, out[a][c][q]) = sum over the rows i of adapter a of h[i][q] x[i][c]
 struct ProjFactor {
     const float* h; int rp, rank;
     const void* x; long long ldx; int N;
     void* out; bool by_col;
+    int splits; float* partial;          // workgroups that share an adapter's rows; splits > 1: proj_factor_partial floats
     long long n; int dtype, out_dtype;
     const long long* offsets; int segments; const int* ids; int adapters;
 };

@@ -2090,17 +2090,20 @@ static bool blocks_overlap(const void* p, int64_t pb, const void* q, int64_t qb)
 }
 
 // Workspace of an adapted call over n rows, in this order: the adapter of each row, the parts of the low-rank intermediate that the output takes up, their row
-// scales, and, backward, both intermediates in fp32 for the factors' gradients.
+// scales, and, backward, both intermediates in fp32 for the factors' gradients and the partial sums of both.
 struct ProjWork {
-    int64_t rows, parts, scale, f32, all;       // rows: the adapter of each row
-    int rp32;
+    int64_t rows, parts, scale, f32, da, db, all;       // rows: the adapter of each row
+    int rp32, splits;
     ProjWork(const vdb_projection* p, int64_t n, bool backward) {
         rp32 = proj_rank_pad(p->rank, VDB_F32);
         parts = (int64_t)round_up((size_t)n * proj_parts(p->dtype) * proj_rank_pad(p->rank, p->dtype) * (p->dtype == VDB_F32 ? 4 : 2), 256);
         scale = p->dtype == VDB_F16 ? (int64_t)round_up((size_t)n * 4, 256) : 0;
         f32 = backward ? (int64_t)round_up((size_t)n * rp32 * 4, 256) : 0;
         rows = (int64_t)round_up((size_t)n * 4, 256);
-        all = rows + parts + scale + 2 * f32;
+        splits = proj_factor_splits(n, p->adapters);
+        da = backward ? proj_factor_partial(splits, p->adapters, (int)p->rank, p->dim_in) * 4 : 0;
+        db = backward ? proj_factor_partial(splits, p->adapters, (int)p->rank, p->dim_out) * 4 : 0;
+        all = rows + parts + scale + 2 * f32 + da + db;
     }
 };
 
@@ -2310,8 +2313,10 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
         ProjFactor f{};
         f.rp = wk.rp32; f.rank = p->rank; f.n = n; f.dtype = p->dtype; f.out_dtype = p->out_dtype;
         f.offsets = (const long long*)offsets; f.segments = (int)requests; f.ids = adapter_ids; f.adapters = p->adapters;
+        f.splits = wk.splits; f.partial = h32 + wk.f32 / 4;
         f.h = g32; f.x = x; f.ldx = ldx; f.N = (int)p->dim_in; f.out = da; f.by_col = false;
         ProjFactor fb = f;
+        fb.partial = f.partial + wk.da / 4;
         fb.h = h32; fb.x = dy; fb.ldx = lddy; fb.N = (int)p->dim_out; fb.out = db; fb.by_col = true;
         VDB_HIP(launch_proj_factors(f, fb, st));
     }
