@@ -721,3 +721,11 @@ def test_requests_that_meet_in_a_tile(engine, n, din, dout, rank, dtype, out):
             other[b:e] = False
     assert torch.equal(got.cpu()[other], clean.cpu()[other])
     assert not torch.isfinite(got.cpu()[~other].float()).all(dim=1).any()
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout", [(5000, 3, 70), (9000, 5, 7), (4500, 70, 2), (2500, 131, 257), (4200, 9, 8), (4200, 67, 12), (3000, 193, 450)])
+def test_sizes_that_are_no_vectors_in_tiles(engine, n, din, dout, dtype, out):
+    """Rows shorter than a vector, and rows that end inside one, where the products are in tiles."""
+    Case(n, din, dout, [2, n // 3, n // 3 + 1, n - 1], dtype, out).check(engine)
+    Case(n, din, dout, [0, n // 2, n], dtype, out, 2, 5, [1, 0], shift=1, pad=1).check(engine)

@@ -43,7 +43,7 @@ __device__ __forceinline__ void pj_shrink_load_x(const ProjShrink& p, const type
     for (int u = 0; u < XS; ++u) {
         const int k = k0 + u * stride + lh * V;
         if constexpr (XV) xa[u] = pj_load_if<pj_u32x4>(k < p.K, x + k);
-        else xa[u] = pj_piece<T>(x + k, p.K - k);
+        else xa[u] = pj_piece<T>(x + k, p.K - k, p.K >= V);
     }
 }
 
@@ -274,8 +274,8 @@ proj_shrink_tile_kernel(ProjShrink p, int tiles) {
         const T* f = (const T*)p.f + (long long)ad * p.f_adapter;
         PJOperand<DT, false, 64> ox;
         PJOperand<DT, FB, RN> of;
-        ox.init((const T*)p.x, p.ldx, r0, p.n);
-        of.init(f, FB ? p.f_k : p.f_rank, 0, p.rank);
+        ox.init((const T*)p.x, p.ldx, r0, p.n, p.K);
+        of.init(f, FB ? p.f_k : p.f_rank, 0, p.rank, p.K);
         long long k = p.K;
         auto next = [&](int stage) {
             const int l = k < KT ? (k > 0 ? (int)k : 0) : KT;

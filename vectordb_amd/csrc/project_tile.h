@@ -51,15 +51,26 @@ typedef pj_u32x4 pj_u32x4_any __attribute__((aligned(2)));
 typedef pj_f32x4 pj_f32x4_any __attribute__((aligned(4)));
 typedef pj_s16x4 pj_s16x4_any __attribute__((aligned(2)));
 
-// The 16 bytes at p of which `left` elements lie in the operand (none: 0 or less), the others zero.
-template <typename T> __device__ __forceinline__ pj_u32x4 pj_piece(const T* p, int left) {
+// The 16 bytes at p of which `left` elements lie in the operand (none: 0 or less), the others zero.  Where the operand's rows hold
+// 16 bytes (`whole`), a part is read as the 16 bytes that end where the row does and moved down, so that every piece is one load
+// without a branch.
+template <typename T> __device__ __forceinline__ int pj_behind(int left) { return left > 0 && left < (int)(16 / sizeof(T)) ? 16 / sizeof(T) - left : 0; }
+template <typename T> __device__ __forceinline__ pj_u32x4 pj_moved(const pj_u32x4& v, int behind) {
+    return __builtin_bit_cast(pj_u32x4, __builtin_bit_cast(unsigned __int128, v) >> (behind * (int)sizeof(T) * 8));
+}
+template <typename T> __device__ __forceinline__ pj_u32x4 pj_piece_unmoved(const T* p, int left) {
+    return pj_load_if<pj_u32x4_any>(left > 0, p - pj_behind<T>(left));
+}
+template <typename T> __device__ __forceinline__ pj_u32x4 pj_piece_by_element(const T* p, int left) {
     constexpr int V = 16 / sizeof(T);
     union { T t[V]; pj_u32x4 v; } r;
-    if (left >= V) r.v = *(const pj_u32x4_any*)p;
-    else
 #pragma unroll
-        for (int j = 0; j < V; ++j) r.t[j] = j < left ? p[j] : (T)0;
+    for (int j = 0; j < V; ++j) r.t[j] = j < left ? p[j] : (T)0;
     return r.v;
+}
+template <typename T> __device__ __forceinline__ pj_u32x4 pj_piece(const T* p, int left, bool whole) {
+    if (whole) return pj_moved<T>(pj_piece_unmoved(p, left), pj_behind<T>(left));
+    return pj_piece_by_element(p, left);
 }
 
 // ------------------------------------------------------------------------------------------- segments
@@ -188,9 +199,12 @@ template <int DT, bool BYK, int R> struct PJOperand {
     long long step[P];
     int kpos[P];                 // k of the piece within a tile
     int rem[P];                  // elements of the piece that lie in the operand's rows (V or 0 if !BYK)
+    bool whole, ragged;          // (through registers) what is contiguous holds 16 bytes; it ends inside one of this tile's pieces
 
     // rows r0 .. r0 + R - 1 of [0, rows), k from 0
-    __device__ __forceinline__ void init(const T* base, long long ld, long long r0, long long rows) {
+    __device__ __forceinline__ void init(const T* base, long long ld, long long r0, long long rows, long long K) {
+        whole = (BYK ? rows : K) >= V;
+        ragged = BYK && r0 + R > rows && rows % V != 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int p = i * PJ_THREADS + (int)threadIdx.x;
@@ -220,18 +234,26 @@ template <int DT, bool BYK, int R> struct PJOperand {
             src[i] += step[i];
         }
     }
-    // the same for operands of any alignment and size, through registers
-    __device__ __forceinline__ void load(pj_u32x4 (&r)[P], int kleft) {
+    // the same for operands of any alignment and size, through registers; W: whole
+    template <bool W> __device__ __forceinline__ void load(pj_u32x4 (&r)[P], int kleft) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int left = BYK ? (kpos[i] < kleft ? rem[i] : 0) : (rem[i] ? kleft - kpos[i] : 0);
-            r[i] = pj_piece<T>(src[i], left);
+            if constexpr (W) r[i] = pj_piece_unmoved(src[i], inside(i, kleft));
+            else r[i] = pj_piece_by_element(src[i], inside(i, kleft));
             src[i] += step[i];
         }
     }
-    __device__ __forceinline__ void put(char* lds, const pj_u32x4 (&r)[P]) const {
+    // the same kleft as when they were loaded
+    template <bool W> __device__ __forceinline__ void put(char* lds, const pj_u32x4 (&r)[P], int kleft) const {
+        const bool parts = W && (BYK ? ragged : kleft < KT);
 #pragma unroll
-        for (int i = 0; i < P; ++i) *(pj_u32x4*)(lds + (i * PJ_THREADS + (int)threadIdx.x) * 16) = r[i];
+        for (int i = 0; i < P; ++i) {
+            const pj_u32x4 v = parts ? pj_moved<T>(r[i], pj_behind<T>(inside(i, kleft))) : r[i];
+            *(pj_u32x4*)(lds + (i * PJ_THREADS + (int)threadIdx.x) * 16) = v;
+        }
+    }
+    __device__ __forceinline__ int inside(int i, int kleft) const {
+        return BYK ? (kpos[i] < kleft ? rem[i] : 0) : (rem[i] ? kleft - kpos[i] : 0);
     }
 };
 
@@ -353,7 +375,8 @@ struct PJProduct {
 
     // VEC: loads straight into LDS.  Otherwise through D sets of registers, loaded D steps ahead and put into the other half of
     // the ring while the current step is multiplied.
-    static constexpr int D = 3;
+    static constexpr int D = R == 128 ? 2 : 3;
+    int kl[D];                   // of k in each
     pj_u32x4 rm[VEC ? 1 : D][VEC ? 1 : PJOperand<DT, MK, R>::P], rn[VEC ? 1 : D][VEC ? 1 : PJOperand<DT, NK, R>::P];
 
     __device__ __forceinline__ int take() {
@@ -373,10 +396,16 @@ struct PJProduct {
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < S - 1; ++i) next(lds, i);
-        } else {
+        } else if (om.whole && on.whole) {
 #pragma unroll
-            for (int i = 0; i < D; ++i) { const int l = take(); om.load(rm[i], l); on.load(rn[i], l); }
+            for (int i = 0; i < D; ++i) load(i);
         }
+    }
+    __device__ __forceinline__ void load(int d) {
+        kl[d] = take();
+        om.template load<true>(rm[d], kl[d]);
+        on.template load<true>(rn[d], kl[d]);
+        asm volatile("" ::: "memory");                              // in this order, for the waits
     }
     __device__ __forceinline__ void multiply(const char* lm, int wm, int wn, pj_f32x4 (&acc)[B][B]) {
         const char* ln = lm + TB;
@@ -404,20 +433,29 @@ struct PJProduct {
             }
             // nothing may still be on its way into LDS when the workgroup's memory goes to another one
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else {
+        } else if (om.whole && on.whole) {
             for (int t = 0; t < tiles; t += D)
 #pragma unroll
-                for (int d = 0; d < D; ++d) {
-                    if (t + d >= tiles) break;
+                for (int d = 0; d < D; ++d) {                       // (steps past the end multiply zeros)
                     char* const buf = lds + ((t + d) & 1) * 2 * TB;
-                    om.put(buf, rm[d]);
-                    on.put(buf + TB, rn[d]);
-                    const int l = take();
-                    om.load(rm[d], l);
-                    on.load(rn[d], l);
+                    om.template put<true>(buf, rm[d], kl[d]);
+                    on.template put<true>(buf + TB, rn[d], kl[d]);
+                    load(d);
                     __syncthreads();                                // (the other half was read a step ago, before the last meeting)
                     multiply(buf, wm, wn, acc);
                 }
+        } else {
+            // rows of less than 16 bytes, element by element
+            for (int t = 0; t < tiles; ++t) {
+                char* const buf = lds + (t & 1) * 2 * TB;
+                const int l = take();
+                om.template load<false>(rm[0], l);
+                om.template put<false>(buf, rm[0], l);
+                on.template load<false>(rn[0], l);
+                on.template put<false>(buf + TB, rn[0], l);
+                __syncthreads();
+                multiply(buf, wm, wn, acc);
+            }
         }
     }
 };
@@ -852,8 +890,8 @@ proj_rows_kernel(PJRowsArgs a) {
     const int col0 = col * R;
     pj_f32x4 acc[B][B] = {};
     PJProduct<DT, false, NK, VEC, R> prod;
-    prod.om.init((const T*)p.x, p.ldx, row0, row1);
-    prod.on.init((const T*)p.w + (long long)seg * p.w_group, p.ldw, col0, p.N);
+    prod.om.init((const T*)p.x, p.ldx, row0, row1, p.K);
+    prod.on.init((const T*)p.w + (long long)seg * p.w_group, p.ldw, col0, p.N, p.K);
     int am[B] = {};
     if constexpr (ADAPT) pj_load_adapters<B>(p, row0 + wm * (R / 2), am);        // before the stages' loads, which return in order
     prod.begin(p.K, pj_lds);
@@ -915,9 +953,9 @@ proj_few_kernel(PJRowsArgs a) {
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * 4 * KS + lh * V;
             if constexpr (VEC) xa[u].v = pj_load_if<pj_u32x4>(k < p.K, x + k);
-            else xa[u].v = pj_piece<T>(x + k, p.K - k);
+            else xa[u].v = pj_piece<T>(x + k, p.K - k, p.K >= V);
             if constexpr (VEC && !NK) wa[u].v = pj_load_if<pj_u32x4>(k < p.K, w + k);
-            else if constexpr (!NK) wa[u].v = pj_piece<T>(w + k, p.K - k);
+            else if constexpr (!NK) wa[u].v = pj_piece<T>(w + k, p.K - k, p.K >= V);
             else
 #pragma unroll
                 for (int j = 0; j < V; ++j) wa[u].t[j] = k + j < p.K ? w[(k + j) * p.ldw] : (T)0;
@@ -980,8 +1018,8 @@ proj_weights_kernel(PJWeightsArgs a) {
     const int m0 = tile / a.n_tiles * R, n0 = tile % a.n_tiles * R;
     pj_f32x4 acc[B][B] = {};
     PJProduct<DT, true, true, VEC, R> prod;
-    prod.om.init((const T*)p.dy + b * p.lddy, p.lddy, m0, p.M);
-    prod.on.init((const T*)p.x + b * p.ldx, p.ldx, n0, p.N);
+    prod.om.init((const T*)p.dy + b * p.lddy, p.lddy, m0, p.M, e - b);
+    prod.on.init((const T*)p.x + b * p.ldx, p.ldx, n0, p.N, e - b);
     prod.begin(e > b ? e - b : 0, pj_lds);
     prod.run(pj_lds, wm, wn, acc);
 #pragma unroll
@@ -1073,6 +1111,7 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
             : pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, PJ_F_ANY, R>, grid, lds, a, st))
     if constexpr (R == 128) {
         // (a factor that cannot be read in vectors would spill here)
+        if constexpr (DT != VDB_F32) if (!vec) return pj_launch(proj_rows_kernel<DT, ODT, false, false, false, PJ_F_ANY, R>, grid, lds, a, st);
 #define PJ_BIG(NK)                                                                                                        \
     (p.row_adapter ? pj_launch(proj_rows_kernel<DT, ODT, NK, true, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st)       \
            : pj_launch(proj_rows_kernel<DT, ODT, NK, true, false, PJ_F_ANY, R>, grid, lds, a, st))
@@ -1124,7 +1163,11 @@ static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
     if (tiles64 <= PJ_FEW_TILES) return pj_few<DT, ODT>(p, vec, st);
     if constexpr (DT == VDB_F32)
         if (((p.n + 63) / 64 + (p.row_adapter ? 0 : p.segments / 2)) * ((p.N + 63) / 64) < PJ_F32_TILES) return pj_rows_sized<DT, ODT, 32>(p, vec, st);
-    const bool big = vec && !pj_small_tiles(tiles) && (!p.row_adapter || pj_factor_vec<DT, V>(p));
+    // Through registers 128 x 128 tiles pay later, and not in fp32 (1025 x 769 bf16, 20 000 rows: 106 us by 64 x 64 and 81 by 128 x 128;
+    // 515 x 387 fp16, 8000 rows, 264 tiles, 21.6 and 23.5, 12 000 rows, 388 tiles, 28.0 and 25.2, 60 000 rows 105 and 85; fp32, 20 000
+    // rows 110 and 129); down the columns of the matrix they would spill.
+    const bool big = vec ? !pj_small_tiles(tiles) && (!p.row_adapter || pj_factor_vec<DT, V>(p))
+                         : DT != VDB_F32 && !p.row_adapter && !p.w_by_k && tiles >= 384;
     return big ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
 }
 
