@@ -1149,8 +1149,8 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
 constexpr long long PJ_FEW_TILES = 64;
 
 // fp32 takes 32 x 32 tiles where 64 x 64 would leave half of the CUs without one (384 x 384, in a graph: 1024 rows, 99 tiles, 10.0 us
-// by 32 x 32 and 13.1 by 64 x 64; 1000 rows of 515 x 387, 126 tiles, 15.0 and 23.4; 2048 rows, 195 tiles, 18.4 and 13.6; 1024 x 768,
-// 192 tiles, 30.4 and 28.1).
+// by 32 x 32 and 13.1 by 64 x 64; 1000 rows of 515 x 387, 126 tiles, 13.4 and 19.7; 2048 rows, 195 tiles, 18.3 and 13.5; 1024 x 768,
+// 192 tiles, 30.4 and 28.2).
 constexpr long long PJ_F32_TILES = 128;
 
 template <int DT, int ODT>
