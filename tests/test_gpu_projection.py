@@ -729,3 +729,30 @@ def test_sizes_that_are_no_vectors_in_tiles(engine, n, din, dout, dtype, out):
     """Rows shorter than a vector, and rows that end inside one, where the products are in tiles."""
     Case(n, din, dout, [2, n // 3, n // 3 + 1, n - 1], dtype, out).check(engine)
     Case(n, din, dout, [0, n // 2, n], dtype, out, 2, 5, [1, 0], shift=1, pad=1).check(engine)
+
+
+def test_shared_factor_gradients_captured_and_replayed(engine):
+    """One adapter's rows divided among workgroups, whose sums go through the workspace: replays beside eager calls."""
+    n = 6000
+    c = Case(n, 136, 200, [0, 2500, 2503, n - 1], "bf16", "f32", 1, 24, [0, 0, 0])
+    dx, da, db = (t.clone() for t in c.backward(engine))
+    ws, size = c.ws(engine, True)
+    out = [output(tuple(t.shape), torch.float32)[1] for t in (dx, da, db)]
+
+    def step(stream, have=size):
+        engine.project_adapted_backward_dev(c.proj, n, c.dy.data_ptr(), 200, c.x.data_ptr(), 136, 3, c.offsets.data_ptr(), c.ids_dev.data_ptr(),
+                                            out[0].data_ptr(), 136, out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), have, stream=stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for t in out:
+            t.fill_(SENTINEL)
+        graph.replay()
+        again = c.backward(engine)
+        torch.cuda.synchronize()
+        for got, eager, want in zip(out, again, (dx, da, db)):
+            assert torch.equal(got, want) and torch.equal(eager, want)
+    with pytest.raises(VdbError) as err:
+        step(0, size - 4)
+    assert err.value.code == _lib.EINVAL
