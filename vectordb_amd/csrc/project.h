@@ -37,6 +37,16 @@ struct ProjRows {
     int rank;
 };
 
+// Can the low-rank factor be read in vectors?  Along a matrix stored column by column (forward) the kernels read 16 bytes of ranks
+// (PJ_F_RANKS), along one stored by k (backward) four columns (PJ_F_COLS).  It goes by the way the launch will read: with one input
+// column, a backward pass has ranks one element apart too.
+inline bool proj_factor_vectors(const ProjRows& p) {
+    const int e = p.dtype == VDB_F32 ? 4 : 2;
+    if (!p.row_adapter) return false;
+    if (p.w_by_k) return p.f_col == 1 && p.N % 4 == 0 && (uintptr_t)p.f % (4 * e) == 0;
+    return p.f_rank == 1 && p.rank % (16 / e) == 0 && (uintptr_t)p.f % 16 == 0;
+}
+
 // h[i][q] = scale[a] * sum_k x[i][k] f[a][q][k] for rows with an adapter; padding is zero
 struct ProjShrink {
     const void* x; long long ldx; long long n; int K;

@@ -667,7 +667,7 @@ __device__ __forceinline__ void pj_low_rank_lanes(const ProjRows& p, long long m
         for (int j = 0; j < C; ++j) {
             const int col = colb + j * 16 + lh * 4;
             if constexpr (F == PJ_F_COLS) {
-                const unsigned at = (unsigned)(col < p.N ? col : p.N - 4) * fcol + (unsigned)q * fr;
+                const unsigned at = (unsigned)(col < p.N ? col : 0) * fcol + (unsigned)q * fr;
                 tx4 fv[V];
 #pragma unroll
                 for (int k = 0; k < V; ++k) fv[k] = pj_load_if<tx4>(q + k < p.rank, f + at + (unsigned)k * fr);
@@ -1087,24 +1087,16 @@ static inline long long pj_filled(long long n, int segments) { return n < segmen
 // and 30 by 64 x 64).
 static inline bool pj_small_tiles(long long tiles128) { return tiles128 < 256; }
 
-// The low-rank factor can be read in vectors: forward its ranks are contiguous, backward its columns.
-template <int DT, int V> static bool pj_factor_vec(const ProjRows& p) {
-    if (!p.row_adapter) return false;
-    return p.f_rank == 1 ? p.rank % V == 0 && (uintptr_t)p.f % 16 == 0
-                         : p.N % 4 == 0 && (uintptr_t)p.f % (4 * PJ<DT>::E) == 0;
-}
-
 template <int DT, int ODT, int R>
 static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     PJRowsArgs a;
     a.p = p;
     a.col_tiles = (p.N + R - 1) / R;
-    constexpr int E = PJ<DT>::E, V = 16 / E;
     a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 16);
     const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + pj_filled(p.n, p.segments);
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
     const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
-    const bool fv = pj_factor_vec<DT, V>(p);
+    const bool fv = proj_factor_vectors(p);
 #define PJ_ROWS(NK, VEC)                                                                              \
     (!p.row_adapter ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY, R>, grid, lds, a, st)     \
      : fv   ? pj_launch(proj_rows_kernel<DT, ODT, NK, VEC, true, NK ? PJ_F_COLS : PJ_F_RANKS, R>, grid, lds, a, st) \
@@ -1129,11 +1121,10 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
     PJRowsArgs a;
     a.p = p;
     a.col_tiles = (p.N + 15) / 16;
-    constexpr int V = 16 / PJ<DT>::E;
     a.vec_out = false;
     const long long row_tiles = p.row_adapter ? (p.n + 15) / 16 : p.n / 16 + pj_filled(p.n, p.segments);
     const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
-    const bool fv = pj_factor_vec<DT, V>(p);
+    const bool fv = proj_factor_vectors(p);
 #define PJ_FEW(NK, VEC)                                                                          \
     (!p.row_adapter ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY>, grid, 0, a, st)      \
      : fv   ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, true, NK ? PJ_F_COLS : PJ_F_RANKS>, grid, 0, a, st) \
@@ -1166,7 +1157,7 @@ static hipError_t pj_rows(const ProjRows& p, hipStream_t st) {
     // Through registers 128 x 128 tiles pay later, and not in fp32 (1025 x 769 bf16, 20 000 rows: 106 us by 64 x 64 and 81 by 128 x 128;
     // 515 x 387 fp16, 8000 rows, 264 tiles, 21.6 and 23.5, 12 000 rows, 388 tiles, 28.0 and 25.2, 60 000 rows 105 and 85; fp32, 20 000
     // rows 110 and 129); down the columns of the matrix they would spill.
-    const bool big = vec ? !pj_small_tiles(tiles) && (!p.row_adapter || pj_factor_vec<DT, V>(p))
+    const bool big = vec ? !pj_small_tiles(tiles) && (!p.row_adapter || proj_factor_vectors(p))
                          : DT != VDB_F32 && !p.row_adapter && !p.w_by_k && tiles >= 384;
     return big ? pj_rows_sized<DT, ODT, 128>(p, vec, st) : pj_rows_sized<DT, ODT, 64>(p, vec, st);
 }
