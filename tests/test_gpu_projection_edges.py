@@ -7,7 +7,28 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_projection import Case                             # noqa: E402
+from test_gpu_projection import Case, close, f64          # noqa: E402
+
+
+def close_in_range(got, want, mag, terms, what):
+    """`close` for results that may lie beyond what fp16 holds: 65 520 is half way between its largest value and the next step, so
+    that the kernel's sum, which is within its own error of the wanted one, may round to infinity from there on."""
+    if got.dtype == torch.float16:
+        g, err = f64(got).reshape(want.shape), (terms + 8) * 2.0 ** -23 * mag
+        inf = np.isinf(g)
+        assert (np.abs(want[inf]) + err[inf] >= 65520).all() and (np.sign(g[inf]) == np.sign(want[inf])).all(), what
+        got, want, mag = got.reshape(want.shape)[torch.from_numpy(~inf).cuda()], want[~inf], mag[~inf]
+    close(got, want, mag, terms, what)
+
+
+def check_in_range(c, engine):
+    """Case.check of an adapted case, for results beyond the range of fp16."""
+    rank = c.proj.rank
+    y, (want, mag) = c.forward(engine), c.want_forward()
+    close_in_range(y, want, mag, c.din + rank, "y")
+    got = c.backward(engine)
+    for name, g, (v, m), t in zip(("dx", "da", "db"), got, c.want_backward(), (c.dout + rank, c.n + max(c.din, c.dout), c.din + c.n)):
+        close_in_range(g, v, m, t, name)
 
 
 def many_adapters(n, adapters):
@@ -27,3 +48,37 @@ def test_adapters_of_narrow_rows(engine, din, dout, n, rank, dtype, out):
     """Rows of 1 to 4 elements, where a factor's ranks and columns both lie one element apart, or hold no vector."""
     off, ids = many_adapters(n, 11)
     Case(n, din, dout, off, dtype, out, 11, rank, ids).check(engine)
+
+
+def spread(c, bits):
+    """Ranks of A x (and of dy B) that span `bits` powers of two, with the other factor making up for it."""
+    r = c.proj.rank
+    e = torch.tensor([float((7 * q) % r) for q in range(r)]).mul_(bits / max(1, r - 1)).sub_(bits / 2).round_()
+    c.a.mul_((2.0 ** e).to(c.dt).cuda()[None, :, None])
+    c.b.mul_((2.0 ** -e).to(c.dt).cuda()[None, None, :])
+    return c
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,rank", [(40, 64, 72, 16), (300, 136, 264, 40), (4300, 128, 264, 16), (17000, 72, 264, 24), (17000, 72, 136, 64)])
+def test_ranks_of_very_different_size(engine, n, din, dout, rank, dtype, out):
+    """A rank that is small in A x but large through B counts as much as any other: the intermediate has the bits of fp32 in every rank."""
+    off, ids = many_adapters(n, 11)
+    check_in_range(spread(Case(n, din, dout, off, dtype, out, 11, rank, ids), 20), engine)
+    check_in_range(spread(Case(n, din, dout, [0, n // 2, n], dtype, out, 2, rank, [1, 0]), 20), engine)
+
+
+@pytest.mark.parametrize("n,requests", [(1, 1), (16, 1), (16, 16), (300, 1), (300, 300), (5000, 1)])
+def test_small_rank_beside_a_large_one(engine, n, requests):
+    """h = (60000, 0.001), B = (2^-20, 30000): the second rank is nearly all of the sum; alone and in a batch."""
+    off = [n * s // requests for s in range(requests + 1)]
+    c = Case(n, 8, 16, off, "f16", "f32", 8, 2, [s % 8 for s in range(requests)], scale=False)
+    c.w.zero_()
+    c.x.zero_()
+    c.x[:, 0] = 1
+    c.a.zero_()
+    c.a[:, 0, 0], c.a[:, 1, 0] = 60000, 0.001
+    c.b[:, :, 0], c.b[:, :, 1] = 2.0 ** -20, 30000
+    c.dy.fill_(0.25)
+    c.check(engine)
+    assert abs(float(c.forward(engine)[n - 1, 3]) - 30.06) < 0.01

@@ -7,21 +7,20 @@ namespace vdb {
 // ------------------------------------------------------------------------------------------- low-rank intermediates
 // Writes four consecutive ranks of one row: as fp32, and as the parts that the low-rank term multiplies.
 template <int DT>
-__device__ __forceinline__ void pj_store_parts(const ProjShrink& p, long long m, int q, int rp, pj_f32x4 v, float down) {
+__device__ __forceinline__ void pj_store_parts(const ProjShrink& p, long long m, int q, int rp, pj_f32x4 v) {
     if (p.h32 && q < p.rp32) *(pj_f32x4*)(p.h32 + m * p.rp32 + q) = v;
     if (!p.h) return;
     if constexpr (DT == VDB_F32) *(pj_f32x4*)((float*)p.h + m * rp + q) = v;
     else {
         constexpr int NP = proj_parts(DT);
         unsigned short* o = (unsigned short*)p.h + m * (NP * rp) + q;
-        if constexpr (DT == VDB_F16) v = v * down;
 #pragma unroll
         for (int u = 0; u < NP; ++u) {
             pj_s16x4 s;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[j] = (short)pj_from_f32<DT>(v[j]);
-                const float rest = v[j] - pj_to_f32<DT>((unsigned short)s[j]);
+                s[j] = (short)pj_from_f32<VDB_BF16>(v[j]);
+                const float rest = v[j] - pj_to_f32<VDB_BF16>((unsigned short)s[j]);
                 v[j] = rest == rest ? rest : 0.f;            // an infinity leaves nothing for the later parts
             }
             *(pj_s16x4*)(o + u * rp) = s;
@@ -116,28 +115,13 @@ template <int DT, int NRB>
 __device__ __forceinline__ void pj_shrink_store(const ProjShrink& p, long long m, bool mine, int ad, pj_f32x4 (&acc)[NRB]) {
     const int lh = (threadIdx.x & 63) >> 4, rp = proj_rank_pad(p.rank, DT);
     const float sc = p.scale ? p.scale[ad] : 1.f;
-    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < NRB; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc[i][j] = i * 16 + lh * 4 + j < p.rank ? sc * acc[i][j] : 0.f;
-            const float size = fabsf(acc[i][j]);
-            if (size < __builtin_huge_valf()) most = fmaxf(most, size);
-        }
-    float down = 1.f;
-    if constexpr (DT == VDB_F16) {
-        // a power of two that brings the row's largest finite entry to 1/2..1 (1 where that entry is next to the limits of fp32)
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const int ex = (int)(__float_as_uint(most) >> 23);
-        const bool scaled = ex > 2 && ex < 253;
-        down = scaled ? __uint_as_float((unsigned)(253 - ex) << 23) : 1.f;      // 2^(126 - ex)
-        if (p.h_scale && lh == 0 && mine) p.h_scale[m] = scaled ? __uint_as_float((unsigned)(ex + 1) << 23) : 1.f;
-    }
+        for (int j = 0; j < 4; ++j) acc[i][j] = i * 16 + lh * 4 + j < p.rank ? sc * acc[i][j] : 0.f;
     if (mine) {
 #pragma unroll
-        for (int i = 0; i < NRB; ++i) if (i * 16 < rp) pj_store_parts<DT>(p, m, i * 16 + lh * 4, rp, acc[i], down);
+        for (int i = 0; i < NRB; ++i) if (i * 16 < rp) pj_store_parts<DT>(p, m, i * 16 + lh * 4, rp, acc[i]);
     }
 }
 

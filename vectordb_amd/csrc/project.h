@@ -12,9 +12,11 @@ constexpr int PROJ_MAX_RANK = 128;
 // Workgroups that the gradient of the matrices is divided into where its output tiles are fewer (32 768 rows of 8 groups, 1024 x 768
 // bf16, whole backward pass: 287 us with 256, 206 with 512, 194 with 768, 204 with 1024).
 constexpr int PJ_SPLIT_WGS = 768;
-// A low-rank intermediate h [n, rank], fp32, is handed to the kernel that multiplies it as parts of the rows' type that add up
-// to it: rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks for 16-bit types, 16 for fp32).
-__host__ __device__ constexpr int proj_parts(int dtype) { return dtype == VDB_F32 ? 1 : dtype == VDB_BF16 ? 3 : 2; }
+// A low-rank intermediate h [n, rank], fp32, is handed to the kernel that multiplies it as it is beside fp32 rows, and as three bf16
+// parts that add up to it beside 16-bit ones (three times 8 bits, and each part with an exponent of its own: parts in fp16 would lose
+// the small ranks of a row beside its large ones): rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks
+// for 16-bit types, 16 for fp32).
+__host__ __device__ constexpr int proj_parts(int dtype) { return dtype == VDB_F32 ? 1 : 3; }
 __host__ __device__ constexpr int proj_rank_pad(int rank, int dtype) {
     return dtype == VDB_F32 ? (rank + 15) / 16 * 16 : (rank + 31) / 32 * 32;
 }
@@ -32,7 +34,6 @@ struct ProjRows {
     // low-rank term: y_i += sum_q h[i][q] f[row_adapter[i]][column][q]; null: none
     const int* row_adapter;              // [n], -1: none
     const void* h;                       // [n][proj_parts][proj_rank_pad]
-    const float* h_scale;                // fp16: [n], what the parts of a row have to be multiplied with
     const void* f; long long f_adapter, f_col, f_rank;       // strides in elements
     int rank;
 };
@@ -52,7 +53,7 @@ struct ProjShrink {
     const void* x; long long ldx; long long n; int K;
     const void* f; long long f_adapter, f_rank, f_k;
     const float* scale;
-    void* h; float* h_scale;             // parts, see ProjRows; null: not wanted
+    void* h;                             // parts, see ProjRows; null: not wanted
     int* row_adapter;                    // [n]: the adapter of each row, -1: none; may be null
     float* h32; int rp32;                // [n][rp32] fp32; null: not wanted
     int rank, dtype;

@@ -539,9 +539,10 @@ template <int DT> struct PJWide {
 };
 
 // ------------------------------------------------------------------------------------------- low-rank term
-// The term h f^T of a wave's block, before the main product.  The fp32 intermediate h comes in parts of the rows' type that add up
-// to it (bf16: three; fp16: two, with a power of two for each row that brings its largest entry to 1/2..1, as fp16 could
-// not hold it), so that no way below rounds h:
+// The term h f^T of a wave's block, before the main product.  Beside 16-bit rows the fp32 intermediate h comes in three bf16 parts
+// that add up to it, so that no way below rounds h; a factor in fp16 is taken apart into two bf16 parts, which hold its 11 bits, as
+// it is multiplied.  (Six products instead of two of fp16 parts, whose range is too small: a rank 2^-20 of its row's largest kept 5
+// bits.  1024 x 768 fp16, 32 768 rows of 48 requests, rank 64: 110 us against 102, 108 without the product of the smallest parts.)
 //   one adapter for all of the wave's rows, or a few and ranks of one step: the matrix unit, all rows by each of them, taken over
 //     as below;
 //   few adapters in 16 rows (two, or one for each 12 ranks): the matrix unit, all 16 rows by one adapter, taken over by the
@@ -563,6 +564,36 @@ __device__ __forceinline__ void pj_settle(pj_f32x4& t) { asm volatile("s_nop 15"
 template <typename T> __device__ __forceinline__ T pj_entry(const T* f, unsigned at) {
     return *(const T*)((const char*)f + at * (unsigned)sizeof(T));
 }
+
+// t += f h^T over one step of ranks, the products of the smallest parts first.
+template <int DT> struct PJFactorParts {
+    pj_u32x4 hi;
+    __device__ __forceinline__ explicit PJFactorParts(const pj_u32x4& f) : hi(f) {}
+    __device__ __forceinline__ void multiply(const pj_u32x4 (&h)[proj_parts(DT)], pj_f32x4& t) const {
+#pragma unroll
+        for (int u = proj_parts(DT) - 1; u >= 0; --u) t = pj_mfma<DT>(hi, h[u], t);
+    }
+};
+template <> struct PJFactorParts<VDB_F16> {
+    pj_u32x4 hi, lo;
+    // the first 8 bits, cut, and the other 3
+    __device__ __forceinline__ explicit PJFactorParts(const pj_u32x4& f) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float a = pj_to_f32<VDB_F16>((unsigned short)f[w]), b = pj_to_f32<VDB_F16>((unsigned short)(f[w] >> 16));
+            const unsigned ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
+            hi[w] = __builtin_amdgcn_perm(ub, ua, 0x07060302);               // the upper halves of both
+            lo[w] = __builtin_amdgcn_perm(__float_as_uint(b - __uint_as_float(ub)), __float_as_uint(a - __uint_as_float(ua)), 0x07060302);
+        }
+    }
+    __device__ __forceinline__ void multiply(const pj_u32x4 (&h)[3], pj_f32x4& t) const {
+#pragma unroll
+        for (int u = 2; u >= 0; --u) {
+            t = pj_mfma<VDB_BF16>(lo, h[u], t);
+            t = pj_mfma<VDB_BF16>(hi, h[u], t);
+        }
+    }
+};
 
 // 16 rows by one adapter on the matrix unit; t: lane's row by columns colb + 16 j + 4 (l / 16) + 0..3
 template <int DT, int F, int C>
@@ -588,8 +619,7 @@ __device__ __forceinline__ void pj_low_rank_block(const ProjRows& p, long long m
             else
 #pragma unroll
                 for (int u = 0; u < V; ++u) { const T e = pj_entry(f, r + u < p.rank ? at + (unsigned)u * fr : 0u); fv.t[u] = r + u < p.rank ? e : (T)0; }
-#pragma unroll
-            for (int u = NP - 1; u >= 0; --u) t[j] = pj_mfma<DT>(fv.v, hv[u], t[j]);
+            PJFactorParts<DT>(fv.v).multiply(hv, t[j]);
             if constexpr (F != PJ_F_RANKS) asm volatile("" ::: "memory");       // one block's loads at a time: registers
         }
     }
@@ -627,19 +657,13 @@ __device__ __forceinline__ void pj_low_rank_all(const ProjRows& p, long long row
 #pragma unroll
             for (int u = 0; u < NP; ++u) hv[i][u] = *(const pj_u32x4*)(h + (long long)i * 16 * (NP * rp) + u * rp + q + lh * V);
 #pragma unroll
-        for (int i = 0; i < B; ++i)
+        for (int j = 0; j < C; ++j) {
+            const PJFactorParts<DT> fp(fv[j].v);
 #pragma unroll
-            for (int j = 0; j < C; ++j)
-#pragma unroll
-                for (int u = NP - 1; u >= 0; --u) acc[i][j] = pj_mfma<DT>(fv[j].v, hv[i][u], acc[i][j]);
-    }
-    if constexpr (DT == VDB_F16)
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const float sc = p.h_scale[row + i * 16 + li];
-#pragma unroll
-            for (int j = 0; j < C; ++j) acc[i][j] = acc[i][j] * sc;
+            for (int i = 0; i < B; ++i) fp.multiply(hv[i], acc[i][j]);
+            if constexpr (DT == VDB_F16) __builtin_amdgcn_sched_barrier(0);     // the parts of one block of columns at a time: registers
         }
+    }
 }
 
 // Every lane its own row's adapter: t += h[m] f[a]^T for its four columns of each block, ranks q0, q0 + qs, ... in steps of V
@@ -661,7 +685,7 @@ __device__ __forceinline__ void pj_low_rank_lanes(const ProjRows& p, long long m
             union { T t[V]; pj_u32x4 v; } hv;
             hv.v = *(const pj_u32x4*)(h + u * rp + q);
 #pragma unroll
-            for (int k = 0; k < V; ++k) hq[k] += pj_to_f32<DT>(hv.t[k]);
+            for (int k = 0; k < V; ++k) hq[k] += pj_to_f32<DT == VDB_F32 ? VDB_F32 : VDB_BF16>(hv.t[k]);
         }
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -730,28 +754,24 @@ __device__ __forceinline__ void pj_low_rank_each(const ProjRows& p, long long ro
 #pragma unroll
                 for (int u = 0; u < V; ++u) { const T e = pj_entry(f, r + u < p.rank ? at + (unsigned)u * fr : 0u); fv[j].t[u] = r + u < p.rank ? e : (T)0; }
         }
+        constexpr int CG = DT == VDB_F16 && C > 2 ? 2 : C;     // blocks of columns at a time: the parts of an fp16 factor take registers
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            if (__ballot(am[i] == ad) == 0) continue;
-            pj_f32x4 t[C] = {};
+        for (int c = 0; c < C; c += CG) {
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
+            for (int i = 0; i < B; ++i) {
+                if (__ballot(am[i] == ad) == 0) continue;
+                pj_f32x4 t[CG] = {};
 #pragma unroll
-                for (int u = NP - 1; u >= 0; --u) t[j] = pj_mfma<DT>(fv[j].v, hv[i][u], t[j]);
-                if constexpr (DT == VDB_F32) pj_settle(t[j]);
+                for (int j = 0; j < CG; ++j) {
+                    PJFactorParts<DT>(fv[c + j].v).multiply(hv[i], t[j]);
+                    if constexpr (DT == VDB_F32) pj_settle(t[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < CG; ++j) if (am[i] == ad) acc[i][c + j] = t[j];
             }
-#pragma unroll
-            for (int j = 0; j < C; ++j) if (am[i] == ad) acc[i][j] = t[j];
+            if constexpr (CG < C) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if constexpr (DT == VDB_F16)
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const long long m = row + i * 16 + li;
-            const float sc = am[i] >= 0 ? p.h_scale[m] : 1.f;
-#pragma unroll
-            for (int j = 0; j < C; ++j) acc[i][j] = acc[i][j] * sc;
-        }
 }
 
 // Adapters of B blocks of 16 rows (lane l: row + 16 i + l % 16); -1: none.
@@ -818,9 +838,8 @@ __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, in
             pj_low_rank_lanes<DT, F, C>(p, mc, colb, am[i], wave * V, waves * V, t);
         }
         if (am[i] >= 0) {
-            const float sc = DT == VDB_F16 ? p.h_scale[mc] : 1.f;
 #pragma unroll
-            for (int j = 0; j < C; ++j) acc[i][j] = DT == VDB_F16 ? t[j] * sc : t[j];
+            for (int j = 0; j < C; ++j) acc[i][j] = t[j];
         }
     }
 }

@@ -2089,21 +2089,20 @@ static bool blocks_overlap(const void* p, int64_t pb, const void* q, int64_t qb)
     return p && q && pb > 0 && qb > 0 && (uintptr_t)p < (uintptr_t)q + (uintptr_t)qb && (uintptr_t)q < (uintptr_t)p + (uintptr_t)pb;
 }
 
-// Workspace of an adapted call over n rows, in this order: the adapter of each row, the parts of the low-rank intermediate that the output takes up, their row
-// scales, and, backward, both intermediates in fp32 for the factors' gradients and the partial sums of both.
+// Workspace of an adapted call over n rows, in this order: the adapter of each row, the parts of the low-rank intermediate that the
+// output takes up, and, backward, both intermediates in fp32 for the factors' gradients and the partial sums of both.
 struct ProjWork {
-    int64_t rows, parts, scale, f32, da, db, all;       // rows: the adapter of each row
+    int64_t rows, parts, f32, da, db, all;       // rows: the adapter of each row
     int rp32, splits;
     ProjWork(const vdb_projection* p, int64_t n, bool backward) {
         rp32 = proj_rank_pad(p->rank, VDB_F32);
         parts = (int64_t)round_up((size_t)n * proj_parts(p->dtype) * proj_rank_pad(p->rank, p->dtype) * (p->dtype == VDB_F32 ? 4 : 2), 256);
-        scale = p->dtype == VDB_F16 ? (int64_t)round_up((size_t)n * 4, 256) : 0;
         f32 = backward ? (int64_t)round_up((size_t)n * rp32 * 4, 256) : 0;
         rows = (int64_t)round_up((size_t)n * 4, 256);
         splits = proj_factor_splits(n, p->adapters);
         da = backward ? proj_factor_partial(splits, p->adapters, (int)p->rank, p->dim_in) * 4 : 0;
         db = backward ? proj_factor_partial(splits, p->adapters, (int)p->rank, p->dim_out) * 4 : 0;
-        all = rows + parts + scale + 2 * f32 + da + db;
+        all = rows + parts + 2 * f32 + da + db;
     }
 };
 
@@ -2145,10 +2144,10 @@ static hipError_t proj_adapted(const vdb_projection* p, int64_t n, const void* x
     s.x = x; s.ldx = ldx; s.n = n; s.K = (int)p->dim_in; s.dtype = p->dtype;
     s.f = p->a; s.f_adapter = p->rank * p->dim_in; s.f_rank = p->dim_in; s.f_k = 1;
     s.scale = p->scale; s.rank = p->rank;
-    s.row_adapter = (int*)ws; s.h = (char*)ws + wk.rows; s.h_scale = (float*)((char*)ws + wk.rows + wk.parts);
+    s.row_adapter = (int*)ws; s.h = (char*)ws + wk.rows;
     s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = ids; s.adapters = p->adapters;
     ProjRows r = proj_forward(p, n, x, ldx, offsets, requests, y, ldy, out_dtype);
-    r.w_group = 0; r.row_adapter = s.row_adapter; r.h = s.h; r.h_scale = s.h_scale; r.rank = p->rank;
+    r.w_group = 0; r.row_adapter = s.row_adapter; r.h = s.h; r.rank = p->rank;
     r.f = p->b; r.f_adapter = p->dim_out * p->rank; r.f_col = p->rank; r.f_rank = 1;
     return launch_proj_adapted(r, s, st);
 }
@@ -2282,22 +2281,22 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     if ((rc = enter())) return rc;
     hipStream_t st = (hipStream_t)stream;
     char* const ws = (char*)workspace;
-    float* const g32 = (float*)(ws + wk.rows + wk.parts + wk.scale);
-    float* const h32 = (float*)(ws + wk.rows + wk.parts + wk.scale + wk.f32);
+    float* const g32 = (float*)(ws + wk.rows + wk.parts);
+    float* const h32 = (float*)(ws + wk.rows + wk.parts + wk.f32);
     ProjShrink s{};
     s.n = n; s.dtype = p->dtype; s.scale = p->scale; s.rank = p->rank; s.rp32 = wk.rp32;
     s.offsets = (const long long*)offsets; s.segments = (int)requests; s.ids = adapter_ids; s.adapters = p->adapters;
     // g = s dy B
     s.x = dy; s.ldx = lddy; s.K = (int)p->dim_out;
     s.f = p->b; s.f_adapter = p->dim_out * p->rank; s.f_rank = 1; s.f_k = p->rank;
-    s.row_adapter = dx ? (int*)ws : nullptr; s.h = dx ? ws + wk.rows : nullptr; s.h_scale = (float*)(ws + wk.rows + wk.parts);
+    s.row_adapter = dx ? (int*)ws : nullptr; s.h = dx ? ws + wk.rows : nullptr;
     s.h32 = da ? g32 : nullptr;
     if (da) {
         // h = s x A^T, again rather than kept from the forward pass
         ProjShrink t = s;
         t.x = x; t.ldx = ldx; t.K = (int)p->dim_in;
         t.f = p->a; t.f_adapter = p->rank * p->dim_in; t.f_rank = p->dim_in; t.f_k = 1;
-        t.row_adapter = nullptr; t.h = nullptr; t.h_scale = nullptr; t.h32 = h32;
+        t.row_adapter = nullptr; t.h = nullptr; t.h32 = h32;
         VDB_HIP(launch_proj_shrink_pair(s, t, st));
     } else {
         VDB_HIP(launch_proj_shrink(s, st));
@@ -2305,7 +2304,7 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     if (dx && n > 0) {
         ProjRows r = proj_forward(p, n, dy, lddy, offsets, requests, dx, lddx, p->out_dtype);
         r.w_group = 0; r.w_by_k = true; r.N = (int)p->dim_in; r.K = (int)p->dim_out;
-        r.row_adapter = (const int*)ws; r.h = ws + wk.rows; r.h_scale = (const float*)(ws + wk.rows + wk.parts); r.rank = p->rank;
+        r.row_adapter = (const int*)ws; r.h = ws + wk.rows; r.rank = p->rank;
         r.f = p->a; r.f_adapter = p->rank * p->dim_in; r.f_col = 1; r.f_rank = p->dim_in;
         VDB_HIP(launch_proj_rows(r, st));
     }
