@@ -82,3 +82,34 @@ def test_small_rank_beside_a_large_one(engine, n, requests):
     c.dy.fill_(0.25)
     c.check(engine)
     assert abs(float(c.forward(engine)[n - 1, 3]) - 30.06) < 0.01
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,requests", [(1, 1), (16, 16), (300, 1), (300, 300), (5000, 1)])
+def test_intermediates_next_to_the_limit_of_fp32(engine, n, requests, dtype):
+    """A x s = 3.3995e38, which bf16 rounds to infinity and fp32 holds; with a small B the result is finite, and so are the gradients."""
+    off = [n * s // requests for s in range(requests + 1)]
+    c = Case(n, 16, 24, off, dtype, "f32", 8, 8, [s % 8 for s in range(requests)])
+    c.x.fill_(0.25)
+    c.a.fill_(0.25)
+    c.s.fill_(3.3995e38)
+    c.b.fill_(2.0 ** -20)
+    c.dy.fill_(2.0 ** -30)
+    assert abs(float(c.s[0]) - 3.3995e38) < 1e33
+    c.w.zero_()
+    y = c.forward(engine)
+    want, mag = c.want_forward()
+    assert 1e33 < abs(want).max() < 1e35
+    close(y, want, mag, 16 + 8, "y")
+    dx = c.backward(engine)[0]
+    (want, mag) = c.want_backward()[0]
+    close(dx, want, mag, 24 + 8, "dx")
+    # and with g = dy B s at the limit
+    c.dy.fill_(0.25)
+    c.b.fill_(0.25)
+    c.a.fill_(2.0 ** -20)
+    c.x.fill_(2.0 ** -20)
+    c.s.fill_(3.3995e38 / float(0.25 * 24 * c.b[0, 0, 0]))
+    dx = c.backward(engine)[0]
+    (want, mag) = c.want_backward()[0]
+    close(dx, want, mag, 24 + 8, "dx")

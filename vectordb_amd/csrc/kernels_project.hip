@@ -19,8 +19,10 @@ __device__ __forceinline__ void pj_store_parts(const ProjShrink& p, long long m,
             pj_s16x4 s;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[j] = (short)pj_from_f32<VDB_BF16>(v[j]);
-                const float rest = v[j] - pj_to_f32<VDB_BF16>((unsigned short)s[j]);
+                // cut, not rounded: three times 8 bits are all of them, and no part of a finite value is infinite
+                const unsigned part = __float_as_uint(v[j]) & 0xffff0000u;
+                s[j] = (short)(part >> 16);
+                const float rest = v[j] - __uint_as_float(part);
                 v[j] = rest == rest ? rest : 0.f;            // an infinity leaves nothing for the later parts
             }
             *(pj_s16x4*)(o + u * rp) = s;

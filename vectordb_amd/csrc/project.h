@@ -14,7 +14,7 @@ constexpr int PROJ_MAX_RANK = 128;
 constexpr int PJ_SPLIT_WGS = 768;
 // A low-rank intermediate h [n, rank], fp32, is handed to the kernel that multiplies it as it is beside fp32 rows, and as three bf16
 // parts that add up to it beside 16-bit ones (three times 8 bits, and each part with an exponent of its own: parts in fp16 would lose
-// the small ranks of a row beside its large ones): rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks
+// the small ranks of a row beside its large ones; only what lies below fp32's smallest normal number, 2^-126, may be lost): rows of proj_parts x proj_rank_pad elements (a step of the matrix unit is 32 ranks
 // for 16-bit types, 16 for fp32).
 __host__ __device__ constexpr int proj_parts(int dtype) { return dtype == VDB_F32 ? 1 : 3; }
 __host__ __device__ constexpr int proj_rank_pad(int rank, int dtype) {
