@@ -113,3 +113,51 @@ def test_intermediates_next_to_the_limit_of_fp32(engine, n, requests, dtype):
     dx = c.backward(engine)[0]
     (want, mag) = c.want_backward()[0]
     close(dx, want, mag, 24 + 8, "dx")
+
+
+def same_with_infinities(got, want, mag, terms, what):
+    """NaN where the formula gives NaN, infinities of the formula's sign, and the finite rest within rounding."""
+    g = f64(got).reshape(want.shape)
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isnan(g), np.isnan(want)), "%s: %d NaN, not %d" % (what, np.isnan(g).sum(), np.isnan(want).sum())
+    assert np.array_equal(g[~fin & ~np.isnan(want)], want[~fin & ~np.isnan(want)]), what
+    close(got.reshape(want.shape)[torch.from_numpy(fin).cuda()], want[fin], mag[fin], terms, what)
+
+
+@pytest.mark.filterwarnings("ignore:invalid value:RuntimeWarning")
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,din,dout,rank,long", [(1, 64, 72, 16, True), (40, 64, 72, 16, False), (90, 33, 41, 5, False), (300, 136, 264, 40, True),
+                                                  (4300, 128, 264, 16, False), (9000, 128, 264, 16, True), (17000, 72, 136, 64, True)])
+def test_infinities_give_what_the_formula_gives(engine, n, din, dout, rank, long, dtype):
+    """Infinite entries of a factor, of a row and of a scale, on every way to the low-rank term."""
+    if long:
+        off, ids = [0, n - n // 2, n], [1, 0]
+    else:
+        off, ids = many_adapters(n, 11)
+    inf = float("inf")
+
+    def check(c, what):
+        (want, mag), got = c.want_forward(), c.forward(engine)
+        same_with_infinities(got, want, mag, c.din + rank, what + " y")
+        (want, mag), got = c.want_backward()[0], c.backward(engine)[0]
+        same_with_infinities(got, want, mag, c.dout + rank, what + " dx")
+
+    c = Case(n, din, dout, off, dtype, "f32", 11, rank, ids)
+    c.b[:, 3, rank // 2] = inf
+    c.b[:, 5, 0] = -inf
+    got = c.forward(engine)
+    same_with_infinities(got, *c.want_forward(), din + rank, "columns of b")
+    c = Case(n, din, dout, off, dtype, "f32", 11, rank, ids)
+    c.a[:, rank // 2, 3] = inf
+    c.a[:, 0, 5] = -inf
+    got = c.backward(engine)[0]
+    same_with_infinities(got, *c.want_backward()[0], dout + rank, "columns of a")
+    # everything positive, so that infinities of one sign meet
+    c = Case(n, din, dout, off, dtype, "f32", 11, rank, ids)
+    for t in (c.x, c.dy, c.w, c.a, c.b, c.s):
+        t.copy_(t.abs() + 0.125)
+    c.x[n // 3, 1] = inf
+    c.dy[n // 3, 1] = inf
+    check(c, "row")
+    c.s[1] = inf
+    check(c, "row and scale")

@@ -641,7 +641,7 @@ __device__ __forceinline__ void pj_low_rank_all(const ProjRows& p, long long row
 #pragma unroll 1
     for (int q = 0; q < p.rank; q += QS) {
         const int r = q + lh * V;
-        pj_u32x4 hv[B][NP];
+        constexpr int BG = DT == VDB_F16 && B > 2 ? 2 : B;     // blocks of rows at a time: the parts of an fp16 factor take registers
         union { T t[V]; pj_u32x4 v; } fv[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -653,15 +653,19 @@ __device__ __forceinline__ void pj_low_rank_all(const ProjRows& p, long long row
                 for (int u = 0; u < V; ++u) { const T e = pj_entry(f, r + u < p.rank ? at + (unsigned)u * fr : 0u); fv[j].t[u] = r + u < p.rank ? e : (T)0; }
         }
 #pragma unroll
-        for (int i = 0; i < B; ++i)
+        for (int g = 0; g < B; g += BG) {
+            pj_u32x4 hv[BG][NP];
 #pragma unroll
-            for (int u = 0; u < NP; ++u) hv[i][u] = *(const pj_u32x4*)(h + (long long)i * 16 * (NP * rp) + u * rp + q + lh * V);
+            for (int i = 0; i < BG; ++i)
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            const PJFactorParts<DT> fp(fv[j].v);
+                for (int u = 0; u < NP; ++u) hv[i][u] = *(const pj_u32x4*)(h + (long long)(g + i) * 16 * (NP * rp) + u * rp + q + lh * V);
 #pragma unroll
-            for (int i = 0; i < B; ++i) fp.multiply(hv[i], acc[i][j]);
-            if constexpr (DT == VDB_F16) __builtin_amdgcn_sched_barrier(0);     // the parts of one block of columns at a time: registers
+            for (int j = 0; j < C; ++j) {
+                const PJFactorParts<DT> fp(fv[j].v);
+#pragma unroll
+                for (int i = 0; i < BG; ++i) fp.multiply(hv[i], acc[g + i][j]);
+            }
+            if constexpr (BG < B) __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -784,13 +788,29 @@ template <int B> __device__ __forceinline__ void pj_load_adapters(const ProjRows
     }
 }
 
+// Is a value infinite or NaN in any lane?
+template <int C> __device__ __forceinline__ float pj_largest(const pj_f32x4 (&t)[C], float z) {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (int n = 0; n < 4; n += 2)                       // (a maximum that a NaN goes through)
+            z = __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(t[j][n]), fabsf(t[j][n + 1])), z);
+    return z;
+}
+template <int C> __device__ __forceinline__ bool pj_any_not_finite(const pj_f32x4 (&t)[C]) {
+    return __ballot(!(pj_largest<C>(t, 0.f) < __builtin_huge_valf())) != 0;
+}
+
 // B blocks of 16 rows from `row`, C of 16 columns from `colb`; am: the rows' adapters.  `waves` > 1: that many waves share the block, and the sum of
 // their accumulators is the term.
+// Where parts are multiplied an infinity times the zero that another part holds is NaN, and infinite parts of both signs are too: what
+// is not finite is worked out again lane by lane, from h put together, and is then what the formula gives.
 template <int DT, int F, int B, int C>
 __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, int colb, const int (&am)[B], pj_f32x4 (&acc)[B][C],
                                             int waves = 1, int wave = 0) {
     constexpr int V = 16 / PJ<DT>::E;
     const int li = threadIdx.x & 15;
+    bool done = false;
     if constexpr (B > 1 && F != PJ_F_ANY) {
         // one adapter for all rows, as long requests have it: its factor is loaded once for all of them
         const int a0 = __builtin_amdgcn_readlane(am[0], 0);
@@ -799,18 +819,24 @@ __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, in
         for (int i = 0; i < B; ++i) same = same && am[i] == a0;
         if (__ballot(!same) == 0) {
             pj_low_rank_all<DT, F, B, C>(p, row, colb, a0, acc);
-            return;
-        }
-        // a few adapters, as where requests meet
-        if (p.rank <= 4 * V) {
+            done = true;
+        } else if (p.rank <= 4 * V) {
+            // a few adapters, as where requests meet
             int v = -1, met = 0;
 #pragma unroll
             for (int i = 0; i < B; ++i) if ((threadIdx.x & 63) >> 4 == i) v = am[i];
             for (unsigned long long left = __ballot(v >= 0); left; ++met) left &= ~__ballot(v == __builtin_amdgcn_readlane(v, __builtin_ctzll(left)));
             if (met <= PJ_EACH_ADAPTER) {
                 pj_low_rank_each<DT, F, B, C>(p, row, colb, am, v, acc);
-                return;
+                done = true;
             }
+        }
+        if (done) {
+            float z = 0.f;
+            if constexpr (DT != VDB_F32)
+#pragma unroll
+                for (int i = 0; i < B; ++i) z = pj_largest<C>(acc[i], z);
+            if (__ballot(!(z < __builtin_huge_valf())) == 0) return;
         }
     }
 #pragma unroll
@@ -818,24 +844,37 @@ __device__ __forceinline__ void pj_low_rank(const ProjRows& p, long long row, in
         const long long m = row + i * 16 + li, mc = m < p.n ? m : p.n - 1;
         const unsigned rows = (unsigned)__ballot(am[i] >= 0) & 0xffffu;
         if (!rows) continue;
-        int met = 0;                                         // adapters in these 16 rows
-        for (unsigned left = rows; left; ++met) left &= ~(unsigned)__ballot(am[i] == __builtin_amdgcn_readlane(am[i], __builtin_ctz(left)));
         pj_f32x4 t[C] = {};
-        if (met <= (p.rank < 32 ? 2 : p.rank / 12)) {
-            int turn = 0;
-            for (unsigned left = rows; left;) {
-                const int ad = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
-                left &= ~(unsigned)__ballot(am[i] == ad);
-                const bool mine = turn == wave;
-                turn = turn + 1 == waves ? 0 : turn + 1;
-                if (!mine) continue;
-                pj_f32x4 u[C] = {};
-                pj_low_rank_block<DT, F, C>(p, mc, colb, ad, u);
+        bool lanes = false;                                  // (of a value that is not finite: alone)
+        if (!done) {
+            int met = 0;                                     // adapters in these 16 rows
+            for (unsigned left = rows; left; ++met) left &= ~(unsigned)__ballot(am[i] == __builtin_amdgcn_readlane(am[i], __builtin_ctz(left)));
+            if (met <= (p.rank < 32 ? 2 : p.rank / 12)) {
+                int turn = 0;
+                for (unsigned left = rows; left;) {
+                    const int ad = __builtin_amdgcn_readlane(am[i], __builtin_ctz(left));
+                    left &= ~(unsigned)__ballot(am[i] == ad);
+                    const bool mine = turn == wave;
+                    turn = turn + 1 == waves ? 0 : turn + 1;
+                    if (!mine) continue;
+                    pj_f32x4 u[C] = {};
+                    pj_low_rank_block<DT, F, C>(p, mc, colb, ad, u);
 #pragma unroll
-                for (int j = 0; j < C; ++j) if (am[i] == ad) t[j] = u[j];
-            }
+                    for (int j = 0; j < C; ++j) if (am[i] == ad) t[j] = u[j];
+                }
+            } else lanes = true;
         } else {
-            pj_low_rank_lanes<DT, F, C>(p, mc, colb, am[i], wave * V, waves * V, t);
+#pragma unroll
+            for (int j = 0; j < C; ++j) t[j] = acc[i][j];
+        }
+        if (lanes || (DT != VDB_F32 && pj_any_not_finite<C>(t))) {
+            pj_f32x4 u[C] = {};
+            pj_low_rank_lanes<DT, F, C>(p, mc, colb, am[i], lanes ? wave * V : 0, lanes ? waves * V : V, u);
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    if (lanes || !(fabsf(t[j][n]) < __builtin_huge_valf())) t[j][n] = u[j][n];
         }
         if (am[i] >= 0) {
 #pragma unroll
