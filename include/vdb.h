@@ -279,7 +279,8 @@ typedef struct vdb_projection {
     const float* scale;          /* [adapters], or NULL: 1 */
 } vdb_projection;
 
-/* Workspace of the calls below, for n rows in `segments` segments; a negative VDB_E* code if the arguments are refused. */
+/* Workspace of the calls below, for n rows in `segments` segments; a negative VDB_E* code if the arguments are refused.  For
+ * `backward` it serves every backward call of the projection: with adapters the factors' and the shared matrix's (the same n). */
 int64_t vdb_projection_workspace_bytes(const vdb_projection* p, int64_t n, int64_t segments, int backward);
 /* y [n, dim_out] = x [n, dim_in] through the matrix of each row's group; offsets [groups + 1]. */
 int vdb_project_grouped_dev(const vdb_projection* p, int64_t n, const void* x, int64_t ldx, const int64_t* offsets,

@@ -161,3 +161,26 @@ def test_infinities_give_what_the_formula_gives(engine, n, din, dout, rank, long
     check(c, "row")
     c.s[1] = inf
     check(c, "row and scale")
+
+
+def test_both_gradients_of_a_handle_with_adapters_in_its_workspace(engine):
+    """The workspace stated for the handle is enough for the gradient of its shared matrix too."""
+    n, din, dout = 16384, 768, 768
+    c = Case(n, din, dout, [0, 5000, 5000, n], "bf16", "f32", 3, 16, [2, 0, 1])
+    ws, size = c.ws(engine, True)
+    dx, dw = torch.empty(n, din, device="cuda"), torch.empty(1, dout, din, device="cuda")
+    whole = torch.tensor([0, n], dtype=torch.int64, device="cuda")
+    engine.project_grouped_backward_dev(c.proj, n, c.dy.data_ptr(), dout, c.x.data_ptr(), din, whole.data_ptr(), dx.data_ptr(), din,
+                                        dw.data_ptr(), ws.data_ptr(), size)
+    torch.cuda.synchronize()
+    assert bool(ws.view(torch.uint8)[size:].view(torch.float32).isnan().all())
+    dy, x, w = f64(c.dy), f64(c.x), f64(c.w)
+    close(dw[0], dy.T @ x, np.abs(dy).T @ np.abs(x), n, "dw")
+    close(dx, dy @ w[0], np.abs(dy) @ np.abs(w[0]), dout, "dx")
+    da, db = torch.empty_like(c.a, dtype=torch.float32), torch.empty_like(c.b, dtype=torch.float32)
+    engine.project_adapted_backward_dev(c.proj, n, c.dy.data_ptr(), dout, c.x.data_ptr(), din, 3, c.offsets.data_ptr(), c.ids_dev.data_ptr(),
+                                        dx.data_ptr(), din, da.data_ptr(), db.data_ptr(), ws.data_ptr(), size)
+    (want, mag), (want_a, mag_a), (want_b, mag_b) = c.want_backward()
+    close(dx, want, mag, dout + 16, "dx")
+    close(da, want_a, mag_a, n + dout, "da")
+    close(db, want_b, mag_b, n + din, "db")

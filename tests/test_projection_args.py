@@ -128,6 +128,26 @@ def test_workspace_sizes():
     assert size(adapter_struct(rank=200), 10, 1, 0) == _lib.EINVAL
 
 
+@pytest.mark.parametrize("n,din,dout,rank", [(16384, 768, 768, 16), (6000, 136, 200, 24), (100, 8, 8, 1), (0, 64, 48, 8), (200000, 1024, 768, 128)])
+def test_one_workspace_serves_both_gradients_of_a_handle_with_adapters(n, din, dout, rank):
+    """The shared matrix's gradient is that of the grouped backward call; the size stated for the handle has to do for it too."""
+    lib = _lib.load()
+    p = adapter_struct(dim_in=din, dim_out=dout, rank=rank)
+    size = lib.vdb_projection_workspace_bytes(C.byref(p), n, 4, 1)
+    alone = lib.vdb_projection_workspace_bytes(C.byref(struct(dim_in=din, dim_out=dout, groups=1)), n, 1, 1)
+    assert size >= alone >= 0
+    # every address far from the others, whatever n
+    far = dict(x=1 << 44, dy=2 << 44, dx=3 << 44, dw=4 << 44, ws=5 << 44, da=6 << 44, db=7 << 44)
+    kw = dict(n=n, ldx=din, lddx=din, lddy=dout, wsb=size, **far)
+    if not _gpu():
+        for fn in ("grouped_backward", "adapted_backward"):
+            assert call(fn, p, **kw) == _lib.ESTATE, (fn, _lib.last_error())
+    # more groups than one: the grouped calls alone take the handle, and their size is stated
+    q = adapter_struct(dim_in=din, dim_out=dout, rank=rank, groups=3)
+    assert lib.vdb_projection_workspace_bytes(C.byref(q), n, 3, 1) == \
+        lib.vdb_projection_workspace_bytes(C.byref(struct(dim_in=din, dim_out=dout)), n, 3, 1)
+
+
 class FakeTensor:
     """What Projection looks at of a tensor."""
     def __init__(self, shape, dtype="torch.bfloat16", device="cuda", index=0, contiguous=True):

@@ -2106,12 +2106,17 @@ struct ProjWork {
     }
 };
 
-static int64_t proj_workspace(const vdb_projection* p, int64_t n, bool adapted, bool backward) {
-    if (adapted) return ProjWork(p, n, backward).all;
-    if (!backward) return 0;
+// partial sums of the gradient of the matrices
+static int64_t proj_grouped_work(const vdb_projection* p, int64_t n) {
     int tile, chunk;
     proj_weights_plan(n, p->groups, (int)p->dim_out, (int)p->dim_in, tile, chunk);
     return chunk > 0 ? (n / chunk + p->groups) * p->dim_out * p->dim_in * (int64_t)sizeof(float) : 0;
+}
+
+// What the header states, and what adapted calls ask for: with adapters, both backward calls of the handle fit into it.
+static int64_t proj_workspace(const vdb_projection* p, int64_t n, bool adapted, bool backward) {
+    const int64_t own = adapted ? ProjWork(p, n, backward).all : 0;
+    return backward ? std::max(own, proj_grouped_work(p, n)) : own;
 }
 
 static int workspace_check(void* ws, int64_t have, int64_t want) {
@@ -2153,7 +2158,7 @@ static hipError_t proj_adapted(const vdb_projection* p, int64_t n, const void* x
 }
 
 int64_t vdb_projection_workspace_bytes(const vdb_projection* p, int64_t n, int64_t segments, int backward) {
-    const bool adapted = p && p->adapters > 0;
+    const bool adapted = p && p->adapters > 0 && p->groups == 1;      // (with more groups the handle serves grouped calls alone)
     const int rc = proj_check(p, n, segments, adapted);
     if (rc) return rc;
     return proj_workspace(p, n, adapted, backward != 0);
@@ -2196,7 +2201,7 @@ int vdb_project_grouped_backward_dev(const vdb_projection* p, int64_t n, const v
     }
     if (dw && (blocks_overlap(dw, dwb, p->w, wn * rx.esize()) || blocks_overlap(dw, dwb, offsets, (p->groups + 1) * (int64_t)8)))
         return fail(VDB_EINVAL, "dw shares memory with an input");
-    const int64_t want = dw ? proj_workspace(p, n, false, true) : 0;
+    const int64_t want = dw ? proj_grouped_work(p, n) : 0;
     if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
     if (want > 0 && (block_overlap(workspace, want, rdy, n) || block_overlap(workspace, want, rx, n) || (dx && block_overlap(workspace, want, rdx, n)) ||
                      blocks_overlap(workspace, want, dw, dwb) || blocks_overlap(workspace, want, p->w, wn * rx.esize())))
@@ -2252,7 +2257,7 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     if (!da != !db) return fail(VDB_EINVAL, "da and db come together");
     if (!dx && !da) return fail(VDB_EINVAL, "dx, da and db are all null");
     const ProjWork wk(p, n, true);
-    const int64_t want = wk.all;
+    const int64_t want = proj_workspace(p, n, true, true);
     const RowsArg rdy{dy, lddy, p->dim_out, p->dtype, "dy"}, rx{x, ldx, p->dim_in, p->dtype, "x"}, rdx{dx, lddx, p->dim_in, p->out_dtype, "dx"};
     const int64_t oe = p->out_dtype == VDB_F32 ? 4 : 2, pairs = (int64_t)p->adapters * p->rank, e = rx.esize();
     const int64_t dab = pairs * p->dim_in * oe, dbb = pairs * p->dim_out * oe;

@@ -208,7 +208,7 @@ class Engine:
         return proj.ptr
 
     def projection_workspace_bytes(self, proj, n: int, segments: int, backward: bool = False) -> int:
-        """Device memory that a call over n rows in `segments` sources or requests works in."""
+        """Device memory that a call over n rows in `segments` sources or requests works in; backward: any backward call of proj."""
         size = self.lib.vdb_projection_workspace_bytes(self._proj(proj), n, segments, 1 if backward else 0)
         if size < 0:
             check(int(size))
