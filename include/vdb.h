@@ -259,8 +259,8 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
  * Numerics.  Products are exact and summed in fp32; a result is rounded once, when it is stored.  The low-rank
  * intermediate A x stays in fp32.  NaN and infinities in one row or adapter reach only the rows that use it.
  *
- * Limits: 2^20 requests, and rows, columns and groups such that no launch needs more than 2^23 workgroups (rows / 64 times the
- * longer dimension / 64); more is refused with VDB_EINVAL.
+ * Limits: 2^20 requests; adapted calls 2^27 rows; (n / 64 + groups + 1) times the longer dimension / 64 up to 2^23 - 8; groups times
+ * dim_in / 64 times dim_out / 64 up to 2^23; n / 64 rounded down and the dimensions' quotients up.  More is refused with VDB_EINVAL.  No launch needs more than 2^23 workgroups; the gradients of very many adapters take several launches.
  *
  * Calls enqueue kernels on `stream` and return; they allocate nothing and may be captured into a graph.  `workspace` is device
  * memory of at least vdb_projection_workspace_bytes, aligned to 16 bytes, its contents need not be kept;  calls (and

@@ -7,7 +7,8 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_projection import Case, close, f64          # noqa: E402
+from test_gpu_projection import Case, close, f64                 # noqa: E402
+from vectordb_amd.projection import Projection                  # noqa: E402
 
 
 def close_in_range(got, want, mag, terms, what):
@@ -184,3 +185,55 @@ def test_both_gradients_of_a_handle_with_adapters_in_its_workspace(engine):
     close(dx, want, mag, dout + 16, "dx")
     close(da, want_a, mag_a, n + dout, "da")
     close(db, want_b, mag_b, n + din, "db")
+
+
+def test_gradients_of_more_adapters_than_one_launch_takes(engine):
+    """8192 wide, 40 000 adapters: two launches (32 768 adapters at most in one); adapters on both sides of the border, all others zero."""
+    n, din, dout, adapters, off, ids = 90, 8192, 16, 40000, [0, 20, 21, 60, 88, 90], [0, 32767, 32768, 39999, 32767]
+    gen = torch.Generator(device="cuda").manual_seed(9)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda").to(torch.bfloat16)
+    x, dy, w, a, b = normal(n, din), normal(n, dout), normal(dout, din), normal(adapters, 1, din), normal(adapters, dout, 1)
+    proj = Projection(w, a=a, b=b, out_dtype=torch.float32)
+    offsets, ids_dev = torch.tensor(off, device="cuda"), torch.tensor(ids, dtype=torch.int32, device="cuda")
+    da, db = torch.full_like(a, 7, dtype=torch.float32), torch.full_like(b, 7, dtype=torch.float32)
+    size = engine.projection_workspace_bytes(proj, n, 5, True)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    engine.project_adapted_backward_dev(proj, n, dy.data_ptr(), dout, x.data_ptr(), din, 5, offsets.data_ptr(), ids_dev.data_ptr(), 0, 0,
+                                        da.data_ptr(), db.data_ptr(), ws.data_ptr(), size)
+    used = torch.zeros(adapters, dtype=torch.bool, device="cuda")
+    used[torch.tensor(ids, device="cuda").unique()] = True
+    assert int(used.sum()) == 4 and float(da[~used].abs().max()) == 0 and float(db[~used].abs().max()) == 0
+    for k in sorted(set(ids)):
+        rows = [i for s in range(5) if ids[s] == k for i in range(off[s], off[s + 1])]
+        xr, dr, ak, bk = f64(x[rows]), f64(dy[rows]), f64(a[k]), f64(b[k])
+        close(da[k], (dr @ bk).T @ xr, (np.abs(dr) @ np.abs(bk)).T @ np.abs(xr), len(rows) + dout, "da")
+        close(db[k], dr.T @ (xr @ ak.T), np.abs(dr).T @ (np.abs(xr) @ np.abs(ak).T), len(rows) + din, "db")
+
+
+def test_twelve_million_rows(engine):
+    """More 16-row blocks than a launch takes workgroups for 768 columns.  Values of -1, 0 and 1: every sum is exact in fp32."""
+    n, din, dout, cut = 12_000_003, 768, 8, 5_592_407
+    gen = torch.Generator(device="cuda").manual_seed(12)
+
+    def signs(*shape):
+        return torch.randint(-1, 2, shape, generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    x = torch.empty(n, din, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, n, 1_000_000):
+        x[i:i + 1_000_000] = signs(min(1_000_000, n - i), din)
+    dy, w = signs(n, dout), signs(2, dout, din)
+    proj = Projection(w, out_dtype=torch.float32)
+    offsets = torch.tensor([0, cut, n], device="cuda")
+    y = torch.full((n, dout), 0.5, device="cuda")
+    engine.project_grouped_dev(proj, n, x.data_ptr(), din, offsets.data_ptr(), y.data_ptr(), dout)
+    size = engine.projection_workspace_bytes(proj, n, 2, True)
+    ws, dw = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.full((2, dout, din), 0.5, device="cuda")
+    engine.project_grouped_backward_dev(proj, n, dy.data_ptr(), dout, x.data_ptr(), din, offsets.data_ptr(), 0, 0, dw.data_ptr(), ws.data_ptr(), size)
+    for g, (b, e) in enumerate([(0, cut), (cut, n)]):
+        want, wt = torch.zeros(dout, din, dtype=torch.float64, device="cuda"), w[g].double().t().contiguous()
+        for i in range(b, e, 500_000):
+            r = x[i:min(i + 500_000, e)].double()
+            assert torch.equal(y[i:i + r.shape[0]].double(), r @ wt), i
+            want += dy[i:i + r.shape[0]].double().t().contiguous() @ r
+        assert torch.equal(dw[g].double(), want)

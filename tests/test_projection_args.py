@@ -148,6 +148,21 @@ def test_one_workspace_serves_both_gradients_of_a_handle_with_adapters(n, din, d
         lib.vdb_projection_workspace_bytes(C.byref(struct(dim_in=din, dim_out=dout)), n, 3, 1)
 
 
+@pytest.mark.parametrize("fn", ["grouped", "grouped_backward", "adapted", "adapted_backward"])
+@pytest.mark.parametrize("din,dout,most", [(768, 768, (((1 << 23) - 8) // 12 - 2) * 64 + 63), (1024, 100, (((1 << 23) - 8) // 16 - 2) * 64 + 63),
+                                           (64, 8, 1 << 27), (1, 1, 1 << 27), (65536, 64, (8191 - 2) * 64 + 63)])
+def test_rows_up_to_the_stated_limit(fn, din, dout, most):
+    """One group: (n / 64 + 2) times the longer dimension / 64 up to 2^23 - 8, and 2^27 rows of adapted calls."""
+    p = struct(dim_in=din, dim_out=dout, groups=1) if fn.startswith("grouped") else adapter_struct(dim_in=din, dim_out=dout, adapters=65535, rank=1)
+    if fn.startswith("grouped"):
+        most = (((1 << 23) - 8) // ((max(din, dout) + 63) // 64) - 2) * 64 + 63
+    kw = dict(ldx=din, ldy=dout, lddx=din, lddy=dout, wsb=1 << 43, x=1 << 44, y=8 << 44, dy=2 << 44, dx=3 << 44, dw=4 << 44, ws=5 << 44,
+              da=6 << 44, db=7 << 44)
+    assert call(fn, p, n=most + 1, **kw) == _lib.EINVAL and "too many rows" in _lib.last_error()
+    if not _gpu():
+        assert call(fn, p, n=most, **kw) == _lib.ESTATE, _lib.last_error()
+
+
 class FakeTensor:
     """What Projection looks at of a tensor."""
     def __init__(self, shape, dtype="torch.bfloat16", device="cuda", index=0, contiguous=True):

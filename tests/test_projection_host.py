@@ -22,4 +22,9 @@ def rules(tmp_path_factory):
 
 def test_vectors_of_a_factor_lie_inside_it(rules):
     """Whatever the sizes (one input column among them, where a backward pass has ranks one element apart)."""
-    assert rules.returncode == 0 and " wrong 0" in rules.stdout, rules.stdout + rules.stderr
+    assert rules.returncode == 0 and "factors: cases 172800 wrong 0\n" in rules.stdout, rules.stdout + rules.stderr
+
+
+def test_launches_of_the_largest_calls_stay_within_the_stated_limit(rules):
+    """The sizes that are taken are those that the header states, and none of their launches needs more than 2^23 workgroups."""
+    assert rules.returncode == 0 and "limits: cases" in rules.stdout and rules.stdout.endswith(" wrong 0\n"), rules.stdout + rules.stderr

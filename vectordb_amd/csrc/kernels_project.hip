@@ -474,7 +474,7 @@ proj_factor_kernel(ProjFactor pa, ProjFactor pb) {
     __shared__ pj_f32x4 part[W - 1][4][64];
     const int lane = threadIdx.x & 63, li = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int split = blockIdx.z / 2, all = W * p.splits, mine = split * W + wave;
-    const int n0 = blockIdx.x * 64, ad = blockIdx.y, c0 = n0 + li * 4;
+    const int n0 = blockIdx.x * 64, ad = p.first + blockIdx.y, c0 = n0 + li * 4;
     pj_f32x4 acc[NRB][4] = {};
     // this wave's blocks of 16 rows, one after the other: rows [r, min(r + 16, e))
     int s0 = -64, turn = 0;                // requests looked at; blocks of the adapter met so far, modulo all
@@ -636,21 +636,10 @@ hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st) {
     return pj_launch(proj_weights_sum_kernel<VDB_F16>, grid, 0, p, st);
 }
 
-// Workgroups for the adapters of one block of 16 rows: as many as it meets if all requests were of one length, and a workgroup to
-// a CU.  More are dispatched in vain (1024 rows of 128 requests: 12.4 us with 256 workgroups in all, 15.1 with 1024), fewer
-// leave adapters one after the other (15.8 us with 128).
-static long long shrink_share(long long n, int segments) {
-    const long long blocks = (n + 15) / 16;
-    long long share = segments / blocks;
-    if (share < 256 / blocks) share = 256 / blocks;
-    if (share > segments) share = segments;
-    return share < 1 ? 1 : share > 16 ? 16 : share;
-}
-
 // By 64 rows: from rank 33 and 16 384 rows on, for long requests (rank 64, 1024 wide, 48 requests: 32 768 rows 47 -> 26 us, 8192 rows
 // 22 -> 30; rank 16, 768 wide: 16 384 rows 12 -> 17).
 template <int DT, int NRB> static bool shrink_tiles(const ProjShrink& p) {
-    return NRB >= 4 && p.n >= 16384 && p.n / p.segments >= 128;
+    return NRB >= 4 && p.n >= 16384 && p.n / p.segments >= 128 && proj_shrink_tile_grid(p.n) <= PROJ_MAX_WORKGROUPS;
 }
 
 template <int DT, int NRB>
@@ -660,10 +649,9 @@ static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
     const bool fk = p.f_k == 1 && pj_aligned(p.f, p.f_rank, E, 16) && p.K % V == 0;
     const bool ftile = p.f_rank == 1 && p.f_k == p.rank && p.rank % V == 0 && (uintptr_t)p.f % 16 == 0;
     const bool fr = DT == VDB_F32 ? p.f_rank == 1 : p.f_rank == 1 && p.f_k == p.rank && p.rank % 8 == 0 && (uintptr_t)p.f % 16 == 0;
-    const long long blocks = (p.n + 15) / 16;
     if constexpr (NRB >= 4) if (shrink_tiles<DT, NRB>(p) && xv && (fk || ftile)) {
         const int tiles = (int)((p.n + 63) / 64);
-        const dim3 grid((unsigned)(tiles + blocks));
+        const dim3 grid((unsigned)proj_shrink_tile_grid(p.n));
         const size_t lds = 4 * (pj_tile_bytes(64) + pj_tile_bytes(NRB <= 4 ? 64 : 128));
         auto go = [&](auto kernel) {
             if (lds > 65536) {
@@ -676,8 +664,8 @@ static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
         if (fk) return go(proj_shrink_tile_kernel<DT, NRB, PJ_S_FK>);
         return go(proj_shrink_tile_kernel<DT, NRB, PJ_S_FR>);
     }
-    const long long share = shrink_share(p.n, p.segments);
-    const dim3 grid((unsigned)(blocks * share));
+    const long long share = proj_shrink_share(p.n, p.segments);
+    const dim3 grid((unsigned)proj_shrink_grid(p.n, p.segments));
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, (int)share);
         return hipGetLastError();
@@ -688,17 +676,23 @@ static hipError_t shrink_typed(const ProjShrink& p, hipStream_t st) {
 }
 
 template <int DT, int ODT, int NRB>
-static hipError_t factor_typed(const ProjFactor& p, const ProjFactor& b, hipStream_t st) {
-    const int most = p.N > b.N ? p.N : b.N;
-    const dim3 grid((unsigned)((most + 63) / 64), (unsigned)p.adapters, 2 * p.splits), threads(PJ_FACTOR_WAVES * 64);
+static hipError_t factor_typed(ProjFactor p, ProjFactor b, hipStream_t st) {
+    const int most = p.N > b.N ? p.N : b.N, step = proj_factor_adapters(p.adapters, p.splits, most);
+    const dim3 threads(PJ_FACTOR_WAVES * 64);
     const bool xv = pj_aligned(p.x, p.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && p.N % 4 == 0 &&
                     pj_aligned(b.x, b.ldx, PJ<DT>::E, 4 * PJ<DT>::E) && b.N % 4 == 0;
-    if (xv) hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, true>), grid, threads, 0, st, p, b);
-    else hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, false>), grid, threads, 0, st, p, b);
-    if (p.splits > 1) {
+    for (int first = 0; first < p.adapters; first += step) {
+        p.first = b.first = first;
+        const int left = p.adapters - first;
+        const dim3 grid((unsigned)((most + 63) / 64), (unsigned)(left < step ? left : step), 2 * p.splits);
+        if (xv) hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, true>), grid, threads, 0, st, p, b);
+        else hipLaunchKernelGGL((proj_factor_kernel<DT, ODT, NRB, false>), grid, threads, 0, st, p, b);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((proj_factor_sum_kernel<ODT, NRB>), dim3(grid.x, grid.y, 2 * ((p.rank + 15) / 16)), dim3(256), 0, st, p, b);
+    }
+    if (p.splits > 1) {                                      // (of a few adapters)
+        const dim3 grid((unsigned)((most + 63) / 64), (unsigned)p.adapters, 2 * ((p.rank + 15) / 16));
+        hipLaunchKernelGGL((proj_factor_sum_kernel<ODT, NRB>), grid, dim3(256), 0, st, p, b);
     }
     return hipGetLastError();
 }
@@ -750,12 +744,12 @@ static hipError_t shrink_pair_typed(const ProjShrink& g, const ProjShrink& h, hi
     constexpr int E = PJ<DT>::E, V = 16 / E;
     const bool vec = pj_aligned(g.x, g.ldx, E, 16) && g.K % V == 0 && pj_aligned(h.x, h.ldx, E, 16) && pj_aligned(h.f, h.f_rank, E, 16) &&
                      h.K % V == 0 && (DT == VDB_F32 || (g.rank % 8 == 0 && (uintptr_t)g.f % 16 == 0));
-    if (!vec || shrink_tiles<DT, NRB>(g)) {
+    if (!vec || shrink_tiles<DT, NRB>(g) || 2 * proj_shrink_grid(g.n, g.segments) > PROJ_MAX_WORKGROUPS) {
         const hipError_t e = shrink_typed<DT, NRB>(g, st);
         return e == hipSuccess ? shrink_typed<DT, NRB>(h, st) : e;
     }
-    const long long share = shrink_share(g.n, g.segments);
-    const dim3 grid((unsigned)((g.n + 15) / 16 * share), 2);
+    const long long share = proj_shrink_share(g.n, g.segments);
+    const dim3 grid((unsigned)proj_shrink_grid(g.n, g.segments), 2);
     hipLaunchKernelGGL((proj_shrink_pair_kernel<DT, NRB>), grid, dim3(256), 0, st, g, h, (int)share);
     return hipGetLastError();
 }

@@ -9,6 +9,9 @@
 namespace vdb {
 
 constexpr int PROJ_MAX_RANK = 128;
+// No launch needs more workgroups; sizes that would are refused (proj_sizes_fit), or take several launches.
+constexpr long long PROJ_MAX_WORKGROUPS = 1LL << 23;
+constexpr long long PROJ_MAX_REQUESTS = 1LL << 20, PROJ_MAX_ADAPTED_ROWS = 16 * PROJ_MAX_WORKGROUPS;
 // Workgroups that the gradient of the matrices is divided into where its output tiles are fewer (32 768 rows of 8 groups, 1024 x 768
 // bf16, whole backward pass: 287 us with 256, 206 with 512, 194 with 768, 204 with 1024).
 constexpr int PJ_SPLIT_WGS = 768;
@@ -38,6 +41,20 @@ struct ProjRows {
     int rank;
 };
 
+// Workgroups of the products of the rows by tiles of R x R: each segment that can have rows adds at most one tile to those that the
+// rows alone would fill; a multiple of eight, for the eight XCDs.
+inline long long proj_rows_grid(const ProjRows& p, int R) {
+    const long long tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + (p.n < p.segments ? p.n : p.segments);
+    return (tiles * ((p.N + R - 1) / R) + 7) / 8 * 8;
+}
+
+// Do all launches of a call stay within PROJ_MAX_WORKGROUPS?  The products of the rows and the gradient of the matrices by 64 x 64
+// tiles (smaller ones are for small calls), the low-rank intermediate by 16 rows.
+inline bool proj_sizes_fit(long long n, long long dim_in, long long dim_out, long long groups, bool adapted) {
+    const long long ti = (dim_in + 63) / 64, to = (dim_out + 63) / 64, most = PROJ_MAX_WORKGROUPS;
+    return n / 64 + groups + 1 <= (most - 8) / (ti > to ? ti : to) && groups * ti <= most / to && (!adapted || n <= PROJ_MAX_ADAPTED_ROWS);
+}
+
 // Can the low-rank factor be read in vectors?  Along a matrix stored column by column (forward) the kernels read 16 bytes of ranks
 // (PJ_F_RANKS), along one stored by k (backward) four columns (PJ_F_COLS).  It goes by the way the launch will read: with one input
 // column, a backward pass has ranks one element apart too.
@@ -59,6 +76,20 @@ struct ProjShrink {
     int rank, dtype;
     const long long* offsets; int segments; const int* ids; int adapters;
 };
+
+// Workgroups for the adapters of one block of 16 rows: as many as it meets if all requests were of one length, and a workgroup to
+// a CU.  More are dispatched in vain (1024 rows of 128 requests: 12.4 us with 256 workgroups in all, 15.1 with 1024), fewer
+// leave adapters one after the other (15.8 us with 128).
+inline long long proj_shrink_share(long long n, int segments) {
+    const long long blocks = (n + 15) / 16;
+    long long share = segments / blocks;
+    if (share < 256 / blocks) share = 256 / blocks;
+    if (share > segments) share = segments;
+    return share < 1 ? 1 : share > 16 ? 16 : share;
+}
+// Workgroups of an intermediate by 16 rows, and by 64 rows with the workgroups for those that meet many adapters.
+inline long long proj_shrink_grid(long long n, int segments) { return (n + 15) / 16 * proj_shrink_share(n, segments); }
+inline long long proj_shrink_tile_grid(long long n) { return (n + 63) / 64 + (n + 15) / 16; }
 
 // dw[g][m][c] = sum over the rows i of segment g of dy[i][m] x[i][c]
 struct ProjWeights {
@@ -86,6 +117,13 @@ inline void proj_weights_plan(long long n, int segments, int M, int N, int& tile
     if (c < n) chunk = (int)c;
 }
 
+// Workgroups of the gradient of the matrices by tiles of tm x tn.
+inline long long proj_weights_grid(const ProjWeights& p, int tm, int tn) {
+    const long long tiles = (long long)((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn);
+    const long long items = p.chunk > 0 ? p.n / p.chunk + (p.n < p.segments ? p.n : p.segments) : p.segments;
+    return (items * tiles + 7) / 8 * 8;
+}
+
 // Workgroups that share the rows of an adapter, as many as leave 512 rows to each, and 16 over all adapters: with few adapters
 // there are too few workgroups, with many the ones that find no rows cost more than the others gain (whole backward pass, 768 x
 // 768 bf16, rank 16, alone and shared: 16 384 rows of 1 adapter 174 and 76 us, of 4 adapters 105 and 78, of 24 adapters by two 80
@@ -95,6 +133,11 @@ inline int proj_factor_splits(long long n, int adapters) {
     const long long most = n / 512, want = PJ_FACTOR_SHARES / adapters;
     const long long s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s);
+}
+// Adapters whose gradients one launch takes, of factors with up to `width` columns.
+inline int proj_factor_adapters(int adapters, int splits, long long width) {
+    const long long most = PROJ_MAX_WORKGROUPS / ((width + 63) / 64 * 2 * splits);
+    return (int)(adapters < most ? adapters : most);
 }
 // floats of the partial sums of one factor's gradient
 inline long long proj_factor_partial(int splits, int adapters, int rank, long long N) {
@@ -110,6 +153,7 @@ struct ProjFactor {
     int splits; float* partial;          // workgroups that share an adapter's rows; splits > 1: proj_factor_partial floats
     long long n; int dtype, out_dtype;
     const long long* offsets; int segments; const int* ids; int adapters;
+    int first;                           // adapter of the launch's first workgroups
 };
 
 hipError_t launch_proj_rows(const ProjRows& p, hipStream_t st);

@@ -1138,9 +1138,6 @@ static hipError_t pj_launch(K kernel, dim3 grid, size_t lds, const A& args, hipS
     return hipGetLastError();
 }
 
-// Segments that can have rows: each adds at most one tile to those that the rows alone would fill.
-static inline long long pj_filled(long long n, int segments) { return n < segments ? n : segments; }
-
 // 64 x 64 tiles where 128 x 128 ones would leave CUs without work (bf16, 768 x 768, 8 groups: 8192 rows, 408 tiles of 128 x 128, 18 us
 // and 30 by 64 x 64).
 static inline bool pj_small_tiles(long long tiles128) { return tiles128 < 256; }
@@ -1151,8 +1148,7 @@ static hipError_t pj_rows_sized(const ProjRows& p, bool vec, hipStream_t st) {
     a.p = p;
     a.col_tiles = (p.N + R - 1) / R;
     a.vec_out = pj_aligned(p.y, p.ldy, PJ<ODT>::E, 16);
-    const long long row_tiles = p.row_adapter ? (p.n + R - 1) / R : p.n / R + pj_filled(p.n, p.segments);
-    const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
+    const dim3 grid((unsigned)proj_rows_grid(p, R));
     const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
     const bool fv = proj_factor_vectors(p);
 #define PJ_ROWS(NK, VEC)                                                                              \
@@ -1180,8 +1176,7 @@ static hipError_t pj_few(const ProjRows& p, bool vec, hipStream_t st) {
     a.p = p;
     a.col_tiles = (p.N + 15) / 16;
     a.vec_out = false;
-    const long long row_tiles = p.row_adapter ? (p.n + 15) / 16 : p.n / 16 + pj_filled(p.n, p.segments);
-    const dim3 grid((unsigned)((row_tiles * a.col_tiles + 7) / 8 * 8));
+    const dim3 grid((unsigned)proj_rows_grid(p, 16));
     const bool fv = proj_factor_vectors(p);
 #define PJ_FEW(NK, VEC)                                                                          \
     (!p.row_adapter ? pj_launch(proj_few_kernel<DT, ODT, NK, VEC, false, PJ_F_ANY>, grid, 0, a, st)      \
@@ -1226,13 +1221,12 @@ static hipError_t pj_weights_sized(const ProjWeights& p, bool vec, hipStream_t s
     a.p = p;
     a.m_tiles = (p.M + R - 1) / R;
     a.n_tiles = (p.N + R - 1) / R;
-    const dim3 grid((unsigned)((long long)p.segments * a.m_tiles * a.n_tiles));
+    const dim3 grid((unsigned)proj_weights_grid(p, R, R));
     const size_t lds = vec ? PJRing<R>::BYTES : PJRing<R>::HALVES;
     if (p.chunk > 0) {
-        const dim3 chunks((unsigned)(((p.n / p.chunk + pj_filled(p.n, p.segments)) * a.m_tiles * a.n_tiles + 7) / 8 * 8));
-        if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st);
-        else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, chunks, lds, a, st)
-                        : pj_launch(proj_weights_kernel<DT, ODT, false, true, R>, chunks, lds, a, st);
+        if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, grid, lds, a, st);
+        else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, true, R>, grid, lds, a, st)
+                        : pj_launch(proj_weights_kernel<DT, ODT, false, true, R>, grid, lds, a, st);
     }
     if constexpr (R == 128) return pj_launch(proj_weights_kernel<DT, ODT, true, false, R>, grid, lds, a, st);
     else return vec ? pj_launch(proj_weights_kernel<DT, ODT, true, false, R>, grid, lds, a, st)
@@ -1249,8 +1243,7 @@ static hipError_t pj_weights(const ProjWeights& p, hipStream_t st) {
             a.p = p;
             a.m_tiles = (p.M + PJ_WIDE_M - 1) / PJ_WIDE_M;
             a.n_tiles = (p.N + PJ_WIDE_N - 1) / PJ_WIDE_N;
-            const long long items = p.chunk > 0 ? p.n / p.chunk + pj_filled(p.n, p.segments) : p.segments;
-            const dim3 grid((unsigned)((items * a.m_tiles * a.n_tiles + 7) / 8 * 8));
+            const dim3 grid((unsigned)proj_weights_grid(p, PJ_WIDE_M, PJ_WIDE_N));
             auto go = [&](auto kernel) {
                 const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, PJ_WIDE_BYTES);
                 return e == hipSuccess ? pj_launch(kernel, grid, PJ_WIDE_BYTES, a, st) : e;

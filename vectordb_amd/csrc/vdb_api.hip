@@ -2037,14 +2037,9 @@ static int proj_check(const vdb_projection* p, int64_t n, int64_t segments, bool
         if (p->rank < 1 || p->rank > PROJ_MAX_RANK) return fail(VDB_EINVAL, "rank must be in [1, 128]");
         if (!p->a || !p->b || (uintptr_t)p->a % e || (uintptr_t)p->b % e) return fail(VDB_EINVAL, "a or b is null or not aligned to its type");
         if ((uintptr_t)p->scale % 4) return fail(VDB_EINVAL, "scale is not aligned to its type");
-        if (segments > (1 << 20)) return fail(VDB_EINVAL, "more than 2^20 requests");
+        if (segments > PROJ_MAX_REQUESTS) return fail(VDB_EINVAL, "more than 2^20 requests");
     }
-    // every launch stays within 2^23 workgroups
-    const int64_t lim = (int64_t)1 << 23, td = 64;
-    const int64_t ct = (std::max(p->dim_in, p->dim_out) + td - 1) / td;
-    if (n > (lim - 8) / ct * 16 || (n / td + (adapted ? 1 : p->groups) + 1) * ct > lim - 8 ||
-        (int64_t)p->groups * ((p->dim_in + td - 1) / td) * ((p->dim_out + td - 1) / td) > lim)
-        return fail(VDB_EINVAL, "too many rows or groups for one call");
+    if (!proj_sizes_fit(n, p->dim_in, p->dim_out, p->groups, adapted)) return fail(VDB_EINVAL, "too many rows or groups for one call");
     return VDB_OK;
 }
 
