@@ -252,8 +252,8 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
  * take no part in the other gradients.  Offsets outside [0, n] are cut to it; where they decrease the
  * results are undefined, but nothing outside the operands is read or written.
  *
- * Layout.  Weights are contiguous; rows may be `ld` elements apart, ld >= the row's length.  An output may share no
- * element with an input.  Any sizes and any alignment to the element are taken; rows, matrices and leading
+ * Layout.  Weights are contiguous; rows may be `ld` elements apart, ld >= the row's length.  An output or the
+ * workspace may share no element with an input or with each other.  Any sizes and any alignment to the element are taken; rows, matrices and leading
  * dimensions that are multiples of 16 bytes are the fast ones.
  *
  * Numerics.  Products are exact and summed in fp32; a result is rounded once, when it is stored.  The low-rank

@@ -148,6 +148,22 @@ def test_one_workspace_serves_both_gradients_of_a_handle_with_adapters(n, din, d
         lib.vdb_projection_workspace_bytes(C.byref(struct(dim_in=din, dim_out=dout)), n, 3, 1)
 
 
+@pytest.mark.parametrize("fn,n,at", [(fn, 5000, at) for fn in ("adapted", "adapted_backward") for at in (W, A, B, S, OFF, IDS)] +
+                         [("grouped_backward", 20000, W), ("grouped_backward", 20000, OFF)])
+@pytest.mark.parametrize("part", ["first", "last"])
+def test_a_workspace_that_lies_on_an_input_is_refused(fn, n, at, part):
+    """Whatever a call reads besides rows; the input in the workspace's first and in its last bytes."""
+    p = struct() if fn.startswith("grouped") else adapter_struct()
+    size = _lib.load().vdb_projection_workspace_bytes(C.byref(p), n, 4, int(fn.endswith("backward")))
+    assert size > 1 << 16
+    ws = at if part == "first" else (at - size + 16) // 16 * 16
+    kw = dict(n=n, wsb=size)
+    assert call(fn, p, ws=ws, **kw) == _lib.EINVAL and "workspace shares memory" in _lib.last_error()
+    if not _gpu():
+        # right in front of the input, and not on it
+        assert call(fn, p, ws=(at - size) // 16 * 16, **kw) == _lib.ESTATE, _lib.last_error()
+
+
 @pytest.mark.parametrize("fn", ["grouped", "grouped_backward", "adapted", "adapted_backward"])
 @pytest.mark.parametrize("din,dout,most", [(768, 768, (((1 << 23) - 8) // 12 - 2) * 64 + 63), (1024, 100, (((1 << 23) - 8) // 16 - 2) * 64 + 63),
                                            (64, 8, 1 << 27), (1, 1, 1 << 27), (65536, 64, (8191 - 2) * 64 + 63)])

@@ -2114,10 +2114,37 @@ static int64_t proj_workspace(const vdb_projection* p, int64_t n, bool adapted, 
     return backward ? std::max(own, proj_grouped_work(p, n)) : own;
 }
 
-static int workspace_check(void* ws, int64_t have, int64_t want) {
+// What a call reads besides rows: matrices, factors, scales, offsets and ids.  Neither outputs nor the workspace may lie on it.
+struct ProjInputs {
+    struct { const void* p; int64_t bytes; } block[6];
+    int count;
+    ProjInputs(const vdb_projection* p, int64_t segments, const int64_t* offsets, const int32_t* ids, bool adapted) {
+        const int64_t e = p->dtype == VDB_F32 ? 4 : 2, pairs = (int64_t)p->adapters * p->rank * e;
+        block[0] = {p->w, p->groups * p->dim_in * p->dim_out * e};
+        block[1] = {offsets, (segments + 1) * 8};
+        block[2] = {ids, segments * 4};
+        block[3] = {p->a, pairs * p->dim_in};
+        block[4] = {p->b, pairs * p->dim_out};
+        block[5] = {p->scale, p->adapters * (int64_t)4};
+        count = adapted ? 6 : 2;
+    }
+    bool overlap(const RowsArg& r, int64_t n) const {
+        bool bad = false;
+        for (int i = 0; i < count; ++i) bad = bad || (block[i].p && block_overlap(block[i].p, block[i].bytes, r, n));
+        return bad;
+    }
+    bool overlap(const void* q, int64_t bytes) const {
+        bool bad = false;
+        for (int i = 0; i < count; ++i) bad = bad || blocks_overlap(block[i].p, block[i].bytes, q, bytes);
+        return bad;
+    }
+};
+
+static int workspace_check(void* ws, int64_t have, int64_t want, const ProjInputs& in) {
     if (want == 0) return VDB_OK;
     if (!ws || have < want) return fail(VDB_EINVAL, "workspace of " + std::to_string(have) + " bytes, " + std::to_string(want) + " needed");
     if ((uintptr_t)ws % 16) return fail(VDB_EINVAL, "the workspace is not aligned to 16 bytes");
+    if (in.overlap(ws, want)) return fail(VDB_EINVAL, "the workspace shares memory with an input");
     return VDB_OK;
 }
 
@@ -2166,8 +2193,7 @@ int vdb_project_grouped_dev(const vdb_projection* p, int64_t n, const void* x, i
     if (n > 0) {
         const RowsArg rx{x, ldx, p->dim_in, p->dtype, "x"}, ry{y, ldy, p->dim_out, p->out_dtype, "y"};
         if ((rc = rows_check(rx, n)) || (rc = rows_check(ry, n)) || (rc = segments_check(offsets, nullptr, p->groups, false))) return rc;
-        if (rows_overlap(rx, ry, n) || block_overlap(p->w, (int64_t)p->groups * p->dim_in * p->dim_out * rx.esize(), ry, n) ||
-            block_overlap(offsets, (p->groups + 1) * (int64_t)8, ry, n))
+        if (rows_overlap(rx, ry, n) || ProjInputs(p, p->groups, offsets, nullptr, false).overlap(ry, n))
             return fail(VDB_EINVAL, "y shares memory with an input");
     }
     if ((rc = enter())) return rc;
@@ -2186,20 +2212,20 @@ int vdb_project_grouped_backward_dev(const vdb_projection* p, int64_t n, const v
     const int64_t wn = (int64_t)p->groups * p->dim_in * p->dim_out, dwb = wn * (p->out_dtype == VDB_F32 ? 4 : 2);
     if (dw && (uintptr_t)dw % (p->out_dtype == VDB_F32 ? 4 : 2)) return fail(VDB_EINVAL, "dw is not aligned to its type");
     if ((rc = segments_check(offsets, nullptr, p->groups, false))) return rc;
+    const ProjInputs in(p, p->groups, offsets, nullptr, false);
     if (n > 0) {
         if ((rc = rows_check(rdy, n)) || (dw && (rc = rows_check(rx, n))) || (dx && (rc = rows_check(rdx, n)))) return rc;
-        if (dx && (rows_overlap(rdx, rdy, n) || (dw && (rows_overlap(rdx, rx, n) || block_overlap(dw, dwb, rdx, n))) ||
-                   block_overlap(p->w, wn * rx.esize(), rdx, n) || block_overlap(offsets, (p->groups + 1) * (int64_t)8, rdx, n)))
+        if (dx && (rows_overlap(rdx, rdy, n) || (dw && (rows_overlap(rdx, rx, n) || block_overlap(dw, dwb, rdx, n))) || in.overlap(rdx, n)))
             return fail(VDB_EINVAL, "dx shares memory with an input or with dw");
         if (dw && (block_overlap(dw, dwb, rdy, n) || block_overlap(dw, dwb, rx, n)))
             return fail(VDB_EINVAL, "dw shares memory with an input");
     }
-    if (dw && (blocks_overlap(dw, dwb, p->w, wn * rx.esize()) || blocks_overlap(dw, dwb, offsets, (p->groups + 1) * (int64_t)8)))
+    if (dw && in.overlap(dw, dwb))
         return fail(VDB_EINVAL, "dw shares memory with an input");
     const int64_t want = dw ? proj_grouped_work(p, n) : 0;
-    if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
+    if ((rc = workspace_check(workspace, workspace_bytes, want, in))) return rc;
     if (want > 0 && (block_overlap(workspace, want, rdy, n) || block_overlap(workspace, want, rx, n) || (dx && block_overlap(workspace, want, rdx, n)) ||
-                     blocks_overlap(workspace, want, dw, dwb) || blocks_overlap(workspace, want, p->w, wn * rx.esize())))
+                     blocks_overlap(workspace, want, dw, dwb)))
         return fail(VDB_EINVAL, "the workspace shares memory with another argument");
     if ((rc = enter())) return rc;
     hipStream_t st = (hipStream_t)stream;
@@ -2228,13 +2254,9 @@ int vdb_project_adapted_dev(const vdb_projection* p, int64_t n, const void* x, i
     if (n > 0 && requests > 0) {
         const RowsArg rx{x, ldx, p->dim_in, p->dtype, "x"}, ry{y, ldy, p->dim_out, p->out_dtype, "y"};
         if ((rc = rows_check(rx, n)) || (rc = rows_check(ry, n)) || (rc = segments_check(offsets, adapter_ids, requests, true))) return rc;
-        const int64_t pair = (int64_t)p->adapters * p->rank * rx.esize();
-        if (rows_overlap(rx, ry, n) || block_overlap(p->w, p->dim_in * p->dim_out * rx.esize(), ry, n) ||
-            block_overlap(p->a, pair * p->dim_in, ry, n) || block_overlap(p->b, pair * p->dim_out, ry, n) ||
-            block_overlap(p->scale, p->scale ? p->adapters * (int64_t)4 : 0, ry, n) ||
-            block_overlap(offsets, (requests + 1) * 8, ry, n) || block_overlap(adapter_ids, requests * 4, ry, n))
-            return fail(VDB_EINVAL, "y shares memory with an input");
-        if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
+        const ProjInputs in(p, requests, offsets, adapter_ids, true);
+        if (rows_overlap(rx, ry, n) || in.overlap(ry, n)) return fail(VDB_EINVAL, "y shares memory with an input");
+        if ((rc = workspace_check(workspace, workspace_bytes, want, in))) return rc;
         if (block_overlap(workspace, want, rx, n) || block_overlap(workspace, want, ry, n))
             return fail(VDB_EINVAL, "the workspace shares memory with x or y");
     }
@@ -2254,30 +2276,23 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
     const ProjWork wk(p, n, true);
     const int64_t want = proj_workspace(p, n, true, true);
     const RowsArg rdy{dy, lddy, p->dim_out, p->dtype, "dy"}, rx{x, ldx, p->dim_in, p->dtype, "x"}, rdx{dx, lddx, p->dim_in, p->out_dtype, "dx"};
-    const int64_t oe = p->out_dtype == VDB_F32 ? 4 : 2, pairs = (int64_t)p->adapters * p->rank, e = rx.esize();
+    const int64_t oe = p->out_dtype == VDB_F32 ? 4 : 2, pairs = (int64_t)p->adapters * p->rank;
     const int64_t dab = pairs * p->dim_in * oe, dbb = pairs * p->dim_out * oe;
     if (da && ((uintptr_t)da % oe || (uintptr_t)db % oe)) return fail(VDB_EINVAL, "da or db is not aligned to its type");
     if ((rc = segments_check(offsets, adapter_ids, requests, true))) return rc;
-    const struct { const void* p; int64_t bytes; } in[] = {
-        {p->w, p->dim_in * p->dim_out * e}, {p->a, pairs * p->dim_in * e}, {p->b, pairs * p->dim_out * e},
-        {p->scale, p->scale ? p->adapters * (int64_t)4 : 0}, {offsets, (requests + 1) * 8}, {adapter_ids, requests * 4}};
+    const ProjInputs in(p, requests, offsets, adapter_ids, true);
     if (n > 0) {
         if ((rc = rows_check(rdy, n)) || (da && (rc = rows_check(rx, n))) || (dx && (rc = rows_check(rdx, n)))) return rc;
-        if ((rc = workspace_check(workspace, workspace_bytes, want))) return rc;
+        if ((rc = workspace_check(workspace, workspace_bytes, want, in))) return rc;
         bool bad = block_overlap(workspace, want, rdy, n) || (da && block_overlap(workspace, want, rx, n)) || (dx && block_overlap(workspace, want, rdx, n));
-        if (dx) {
-            bad = bad || rows_overlap(rdx, rdy, n) || (da && (rows_overlap(rdx, rx, n) || block_overlap(da, dab, rdx, n) || block_overlap(db, dbb, rdx, n)));
-            for (const auto& b : in) bad = bad || block_overlap(b.p, b.bytes, rdx, n);
-        }
+        if (dx) bad = bad || rows_overlap(rdx, rdy, n) || in.overlap(rdx, n) ||
+                      (da && (rows_overlap(rdx, rx, n) || block_overlap(da, dab, rdx, n) || block_overlap(db, dbb, rdx, n)));
         if (da) bad = bad || block_overlap(da, dab, rdy, n) || block_overlap(da, dab, rx, n) || block_overlap(db, dbb, rdy, n) ||
                       block_overlap(db, dbb, rx, n) || blocks_overlap(workspace, want, da, dab) || blocks_overlap(workspace, want, db, dbb);
         if (bad) return fail(VDB_EINVAL, "an output or the workspace shares memory with another argument");
     }
-    if (da) {
-        bool bad = blocks_overlap(da, dab, db, dbb);
-        for (const auto& b : in) bad = bad || blocks_overlap(b.p, b.bytes, da, dab) || blocks_overlap(b.p, b.bytes, db, dbb);
-        if (bad) return fail(VDB_EINVAL, "da or db shares memory with another argument");
-    }
+    if (da && (blocks_overlap(da, dab, db, dbb) || in.overlap(da, dab) || in.overlap(db, dbb)))
+        return fail(VDB_EINVAL, "da or db shares memory with another argument");
     if ((rc = enter())) return rc;
     hipStream_t st = (hipStream_t)stream;
     char* const ws = (char*)workspace;
