@@ -262,9 +262,11 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
  * Limits: 2^20 requests; adapted calls 2^27 rows; (n / 64 + groups + 1) times the longer dimension / 64 up to 2^23 - 8; groups times
  * dim_in / 64 times dim_out / 64 up to 2^23; n / 64 rounded down and the dimensions' quotients up.  More is refused with VDB_EINVAL.  No launch needs more than 2^23 workgroups; the gradients of very many adapters take several launches.
  *
- * Calls enqueue kernels on `stream` and return; they allocate nothing and may be captured into a graph.  `workspace` is device
- * memory of at least vdb_projection_workspace_bytes, aligned to 16 bytes, its contents need not be kept;  calls (and
- * captured graphs) that may run at the same time need workspaces of their own. */
+ * The vdb_project_* calls enqueue kernels on `stream` and return; they allocate nothing and may be captured into a graph.
+ * `workspace` is device memory of at least vdb_projection_workspace_bytes, aligned to 16 bytes, its contents need not be kept;
+ * calls (and captured graphs) that may run at the same time need workspaces of their own.  The projected insert and search work in
+ * memory that the library keeps from call to call and enlarges when a call needs more (that waits for the device); they are not for
+ * capture. */
 typedef struct vdb_projection {
     int64_t dim_in, dim_out;     /* 1 .. 65536 */
     int32_t dtype;               /* VDB_F32, VDB_BF16, VDB_F16: type of rows, of incoming gradients and of every weight */
@@ -304,7 +306,8 @@ int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const v
                                      void* workspace, int64_t workspace_bytes, void* stream);
 /* vdb_insert_dev of rows that go through the matrix of their group first (dim_out = the table's dimension; out_dtype is
  * not looked at: the table receives the fp32 sums).  Every row has to have a group: offsets[0] = 0, offsets[groups] = n.
- * Waits for its stream, like vdb_insert_dev. */
+ * Rows pass through memory of insert_buffer_size_gb at most, piece by piece, and appear in the table together.  Waits for its stream,
+ * like vdb_insert_dev. */
 int vdb_insert_projected_dev(const char* name, const vdb_projection* p, int64_t n, const void* x, int64_t ldx,
                              const int64_t* offsets, const int64_t* ids_dev, void* stream);
 /* vdb_search_dev with queries that go through the shared matrix and their request's adapter first (out_dtype is not

@@ -8,7 +8,9 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from test_gpu_projection import Case, close, f64                 # noqa: E402
-from vectordb_amd.projection import Projection                  # noqa: E402
+from vectordb_amd import _lib                                    # noqa: E402
+from vectordb_amd._lib import VdbError                           # noqa: E402
+from vectordb_amd.projection import Projection                   # noqa: E402
 
 
 def close_in_range(got, want, mag, terms, what):
@@ -237,3 +239,77 @@ def test_twelve_million_rows(engine):
             assert torch.equal(y[i:i + r.shape[0]].double(), r @ wt), i
             want += dy[i:i + r.shape[0]].double().t().contiguous() @ r
         assert torch.equal(dw[g].double(), want)
+
+
+def spin(seconds):
+    """Keeps one workgroup of the current stream busy for about that long."""
+    spin.rate = getattr(spin, "rate", None)
+    if spin.rate is None:
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda._sleep(1000)
+        torch.cuda.synchronize()
+        a.record()
+        torch.cuda._sleep(1_000_000)
+        b.record()
+        torch.cuda.synchronize()
+        spin.rate = 1e9 / a.elapsed_time(b)                       # cycles a second
+    torch.cuda._sleep(int(seconds * spin.rate))
+
+
+def test_a_projected_insert_does_not_wait_for_other_streams(engine, table_name):
+    """Warm inserts free and allocate nothing: one returns while another stream is still at work, as a plain insert does."""
+    n, dim = 2000, 64
+    c = Case(n, 48, dim, [0, 700, n], "bf16", "f32")
+    engine.create_table(table_name, dim, _lib.METRIC_IP, _lib.F32)
+    ids = torch.arange(n, dtype=torch.int64, device="cuda")
+    rows = torch.randn(n, dim, device="cuda")
+    mine = torch.cuda.Stream()
+
+    def plain():
+        engine.insert_dev(table_name, n, rows.data_ptr(), ids.data_ptr(), stream=mine.cuda_stream)
+
+    def projected():
+        engine.insert_projected_dev(table_name, c.proj, n, c.x.data_ptr(), 48, c.offsets.data_ptr(), ids.data_ptr(), stream=mine.cuda_stream)
+    engine.reserve(table_name, 1 << 17)
+    plain()
+    projected()
+    for _ in range(8):                                            # streams of one hardware queue wait for each other: another one
+        other, done = torch.cuda.Stream(), torch.cuda.Event()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            spin(0.5)
+            done.record()
+        plain()
+        if done.query():
+            continue
+        projected()
+        assert not done.query(), "the projected insert waited for work of another stream"
+        done.synchronize()
+        assert engine.count(table_name) % n == 0
+        return
+    pytest.skip("every stream shares its hardware queue with this one")
+
+
+@pytest.mark.parametrize("rows_of_a_piece", [1, 100, 333, 1200, 2999])
+def test_projected_insert_in_pieces(engine, table_name, rows_of_a_piece):
+    """An insert larger than the insert buffer: groups that end inside pieces, pieces inside groups; nothing is inserted if the last
+    piece holds a row that is not finite."""
+    n, dim = 3000, 96
+    c = Case(n, 136, dim, [0, 1, 1, 400, 1700, n], "bf16", "f32")
+    engine.create_table(table_name, dim, _lib.METRIC_IP, _lib.F32)
+    ids = torch.arange(n, dtype=torch.int64, device="cuda") * 7 - 3
+    engine.set_option("insert_buffer_size_gb", rows_of_a_piece * dim * 4 / 2.0 ** 30)
+    try:
+        last = c.x[n - 1].clone()
+        c.x[n - 1, 5] = float("inf")
+        with pytest.raises(VdbError) as err:
+            engine.insert_projected_dev(table_name, c.proj, n, c.x.data_ptr(), 136, c.offsets.data_ptr(), ids.data_ptr())
+        assert err.value.code == _lib.EINVAL and engine.count(table_name) == 0
+        c.x[n - 1] = last
+        engine.insert_projected_dev(table_name, c.proj, n, c.x.data_ptr(), 136, c.offsets.data_ptr(), ids.data_ptr())
+    finally:
+        engine.set_option("insert_buffer_size_gb", 1.0)
+    stored, got_ids = engine.fetch_rows(table_name, 0, n)
+    assert np.array_equal(got_ids, ids.cpu().numpy())
+    want, mag = c.want_forward()
+    close(torch.from_numpy(stored), want, mag, 136, "rows")

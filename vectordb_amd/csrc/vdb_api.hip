@@ -11,6 +11,7 @@
 #include <condition_variable>
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -264,6 +265,18 @@ static void release_ws(std::unique_ptr<Workspace>& w, hipStream_t st) {
     std::lock_guard<std::mutex> lk(G.mu);
     G.free_ws.push_back(std::move(w));
 }
+
+// A workspace that goes back to the free ones however the call ends.
+struct HeldWorkspace {
+    std::unique_ptr<Workspace> ws;
+    hipStream_t st;
+    explicit HeldWorkspace(hipStream_t stream) : st(stream) {}
+    int acquire() { return acquire_ws(st, ws); }
+    ~HeldWorkspace() {
+        if (!ws) return;
+        try { release_ws(ws, st); } catch (const std::exception&) {}
+    }
+};
 
 SelGeom sel_geom(int k) {
     SelGeom g;
@@ -1238,12 +1251,20 @@ static int table_stats_update(Table& t, int64_t end, hipStream_t st) {
     return VDB_OK;
 }
 
+// Rows of an insert that are made on its stream piece by piece: rows [first, first + count) of the call into `rows`, which holds
+// `piece` of them.
+struct RowMaker {
+    float* rows;
+    int64_t piece;
+    std::function<hipError_t(int64_t first, int64_t count, hipStream_t st)> make;
+};
+
 // Appends run one at a time per table and beside searches: the new rows are written behind the
 // published row count, the stream is drained, and only then is the count advanced (one atomic
 // store), so a search sees either none or all rows of a call.  A call that meets a row that is not
 // finite in the table's storage type publishes nothing and fails with VDB_EINVAL.
 static int insert_locked(Table& t, int64_t n, const float* rows, const long long* ids,
-                         bool host, bool synth, uint64_t seed, int64_t first_row, hipStream_t user_st) {
+                         bool host, bool synth, uint64_t seed, int64_t first_row, hipStream_t user_st, const RowMaker* maker) {
     int rc;
     if ((rc = table_grow_for(t, n))) return rc;
     const int d = (int)t.dim;
@@ -1256,8 +1277,13 @@ static int insert_locked(Table& t, int64_t n, const float* rows, const long long
     if (synth || !host) {
         hipStream_t st = synth ? G.insert_stream : user_st;
         VDB_HIP(hipMemsetAsync(pending, 0, sizeof(float), st));
-        VDB_HIP(launch_append(t.d_rows, mirror, t.ld16, t.d_ids, t.d_n2, pending, t.d_bad, base, n, d, t.m, t.dtype,
-                              t.metric, synth ? nullptr : rows, synth ? nullptr : ids, seed, first_row, st));
+        const int64_t piece = maker ? maker->piece : n;
+        for (int64_t i0 = 0; i0 < n; i0 += piece) {
+            const int64_t ni = n - i0 < piece ? n - i0 : piece;
+            if (maker) VDB_HIP(maker->make(i0, ni, st));          // (stream order: the last piece has been appended)
+            VDB_HIP(launch_append(t.d_rows, mirror, t.ld16, t.d_ids, t.d_n2, pending, t.d_bad, base + i0, ni, d, t.m, t.dtype,
+                                  t.metric, synth ? nullptr : maker ? maker->rows : rows, synth ? nullptr : ids + i0, seed, first_row, st));
+        }
         VDB_HIP(launch_fold_max(t.d_maxn2, pending, t.d_bad, st));
         VDB_HIP(hipStreamSynchronize(st));
     } else {
@@ -1289,14 +1315,14 @@ static int insert_locked(Table& t, int64_t n, const float* rows, const long long
 }
 
 static int insert_into(Table& t, int64_t n, const float* rows, const long long* ids,
-                       bool host, bool synth, uint64_t seed, int64_t first_row, hipStream_t user_st) {
+                       bool host, bool synth, uint64_t seed, int64_t first_row, hipStream_t user_st, const RowMaker* maker = nullptr) {
     if (t.vmm) {
         {
             // searches keep running: nothing they read moves or changes
             std::shared_lock<std::shared_mutex> tl(t.mu);
             std::lock_guard<std::mutex> il(t.ins_mu);
             if (t.dropped) return fail(VDB_ENOTFOUND, "table was dropped");
-            const int rc = insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st);
+            const int rc = insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st, maker);
             if (rc != VDB_ENOMEM || !t.mirrored()) return rc;
         }
         // out of memory with a mirror in place: the mirror makes room (exclusive lock: no search may be
@@ -1305,15 +1331,15 @@ static int insert_into(Table& t, int64_t n, const float* rows, const long long* 
         std::lock_guard<std::mutex> il(t.ins_mu);
         if (t.dropped) return fail(VDB_ENOTFOUND, "table was dropped");
         table_drop_mirror(t);
-        return insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st);
+        return insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st, maker);
     }
     std::unique_lock<std::shared_mutex> tl(t.mu);
     std::lock_guard<std::mutex> il(t.ins_mu);
     if (t.dropped) return fail(VDB_ENOTFOUND, "table was dropped");
-    int rc = insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st);
+    int rc = insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st, maker);
     if (rc == VDB_ENOMEM && t.mirrored()) {
         table_drop_mirror(t);
-        rc = insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st);
+        rc = insert_locked(t, n, rows, ids, host, synth, seed, first_row, user_st, maker);
     }
     return rc;
 }
@@ -2359,17 +2385,35 @@ int vdb_insert_projected_dev(const char* name, const vdb_projection* p, int64_t 
         bool good = off.front() == 0 && off.back() == n;
         for (size_t i = 1; i < off.size(); ++i) good = good && off[i - 1] <= off[i];
         if (!good) return fail(VDB_EINVAL, "offsets must run from 0 to n without decreasing: every row of an insert needs a group");
-        // the projected rows wait in memory of the call's own: the insert publishes all of them at once
-        void* rows = nullptr;
-        if (hipMalloc(&rows, (size_t)n * t->dim * sizeof(float)) != hipSuccess) {
+        // The rows are projected and appended in pieces of the insert buffer's size, through memory that stays with a workspace:
+        // hipFree would wait for every search in flight.  All of them are published at once.
+        const double fit = G.insert_buffer_gb * 1073741824.0 / ((double)t->dim * sizeof(float));
+        const int64_t most = fit < 1 ? 1 : fit > (double)n ? n : (int64_t)fit;
+        const int64_t pieces = (n + most - 1) / most, piece = (n + pieces - 1) / pieces;
+        const size_t rb = round_up((size_t)piece * t->dim * sizeof(float), 256);
+        HeldWorkspace held(st);
+        if ((rc = held.acquire())) return rc;
+        // each piece's own offsets, relative to its first row
+        std::vector<int64_t> cut;
+        for (int64_t i0 = 0; pieces > 1 && i0 < n; i0 += piece)
+            for (const int64_t o : off) cut.push_back(std::min(std::max(o - i0, (int64_t)0), std::min(piece, n - i0)));
+        DevBuf& mem = held.ws->proj;
+        if (ensure(mem, rb + cut.size() * sizeof(int64_t), held.ws->last_stream)) {
             (void)hipGetLastError();
-            return fail(VDB_ENOMEM, "no memory for " + std::to_string(n) + " projected rows");
+            return fail(VDB_ENOMEM, "no memory for " + std::to_string(piece) + " projected rows");
         }
-        const hipError_t e = launch_proj_rows(proj_forward(p, n, x, ldx, offsets, p->groups, rows, t->dim, VDB_F32), st);
-        rc = e == hipSuccess ? insert_into(*t, n, (const float*)rows, (const long long*)ids_dev, false, false, 0, 0, st)
-                             : fail(VDB_EHIP, std::string("projection: ") + hipGetErrorString(e));
-        (void)hipStreamSynchronize(st);
-        (void)hipFree(rows);
+        int64_t* const cut_dev = (int64_t*)((char*)mem.p + rb);
+        if (pieces > 1) {
+            VDB_HIP(hipMemcpyAsync(cut_dev, cut.data(), cut.size() * sizeof(int64_t), hipMemcpyHostToDevice, st));
+            VDB_HIP(hipStreamSynchronize(st));                   // (host memory of this call)
+        }
+        RowMaker maker{(float*)mem.p, piece, [&](int64_t first, int64_t count, hipStream_t on) {
+            const char* from = (const char*)x + first * ldx * (p->dtype == VDB_F32 ? 4 : 2);
+            const int64_t* o = pieces > 1 ? cut_dev + first / piece * (int64_t)off.size() : offsets;
+            return launch_proj_rows(proj_forward(p, count, from, ldx, o, p->groups, mem.p, t->dim, VDB_F32), on);
+        }};
+        rc = insert_into(*t, n, nullptr, (const long long*)ids_dev, false, false, 0, 0, st, &maker);
+        if (rc) (void)hipStreamSynchronize(st);                  // the caller's rows may still be read
     } catch (const std::exception&) {
         return fail(VDB_ENOMEM, "out of host memory");
     }
@@ -2391,8 +2435,9 @@ int vdb_search_projected_dev(const char* name, const vdb_projection* p, int64_t 
     if (nq == 0) return VDB_OK;
     hipStream_t st = (hipStream_t)stream;
     try {
-        std::unique_ptr<Workspace> ws;
-        if ((rc = acquire_ws(st, ws))) return rc;
+        HeldWorkspace held(st);
+        if ((rc = held.acquire())) return rc;
+        Workspace* const ws = held.ws.get();
         const size_t hb = (size_t)proj_workspace(p, nq, true, false), qb = (size_t)nq * t->dim * sizeof(float);
         rc = ensure(ws->proj, hb + qb, ws->last_stream);
         if (rc == VDB_OK) {
@@ -2407,7 +2452,6 @@ int vdb_search_projected_dev(const char* name, const vdb_projection* p, int64_t 
                 else rc = search_core(*t, nq, q, k, (long long*)out_ids_dev, out_scores_dev, out_counts_dev, st, *ws);
             }
         }
-        release_ws(ws, st);
     } catch (const std::exception&) {
         return fail(VDB_ENOMEM, "out of host memory");
     }
