@@ -313,3 +313,58 @@ def test_projected_insert_in_pieces(engine, table_name, rows_of_a_piece):
     assert np.array_equal(got_ids, ids.cpu().numpy())
     want, mag = c.want_forward()
     close(torch.from_numpy(stored), want, mag, 136, "rows")
+
+
+def guarded(size, guard):
+    """(everything, address of `size` bytes with `guard` bytes of ones on both sides)."""
+    guard = (guard + 255) // 256 * 256
+    buf = torch.full((guard + (size + 255) // 256 * 256 + guard,), 255, dtype=torch.uint8, device="cuda")
+    return buf, buf.data_ptr() + guard, guard
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,off", [
+    (20100, 128, 136, list(range(101)) + [20100]),                           # a hundred groups of one row and a long one
+    (20100, 128, 136, [0] + [20000 + i for i in range(101)]),
+    (193 * 60, 120, 130, [193 * i for i in range(61)]),                      # chunks of one row behind full ones in every group
+    (7000, 67, 515, [0, 3500, 3500, 7000]),
+    (33000, 256, 136, [0, 1, 32999]),
+])
+def test_partial_sums_of_the_matrices_stay_in_the_workspace(engine, n, din, dout, off, dtype, out):
+    c = Case(n, din, dout, off, dtype, out)
+    size = engine.projection_workspace_bytes(c.proj, n, len(off) - 1, True)
+    assert size > 0
+    buf, ws, guard = guarded(size, max(1 << 20, din * dout * 4))
+    dw = torch.empty_like(c.w, dtype=c.out)
+    engine.project_grouped_backward_dev(c.proj, n, c.dy.data_ptr(), dout, c.x.data_ptr(), din, c.offsets.data_ptr(), 0, 0, dw.data_ptr(), ws, size)
+    torch.cuda.synchronize()
+    assert bool((buf[:guard] == 255).all()) and bool((buf[guard + size:] == 255).all())
+    want, mag = c.want_backward()[1]
+    close(dw, want, mag, n, "dw")
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,adapters,rank", [(1, 8, 8, 1, 1), (5000, 131, 257, 3, 100), (9000, 72, 66, 1, 128), (2100, 515, 33, 7, 65),
+                                                      (17000, 64, 136, 2, 70), (300, 65, 63, 40, 128)])
+def test_adapted_calls_stay_in_the_workspace(engine, n, din, dout, adapters, rank, dtype, out):
+    off = [0, n // 5, n // 5, n // 2, n - n // 9]
+    c = Case(n, din, dout, off, dtype, out, adapters, rank, [s % adapters for s in range(4)])
+    want, want_back = c.want_forward(), c.want_backward()
+    for backward in (False, True):
+        size = engine.projection_workspace_bytes(c.proj, n, 4, backward)
+        buf, ws, guard = guarded(size, max(1 << 20, 4 * rank * max(din, dout)))
+        seg = (4, c.offsets.data_ptr(), c.ids_dev.data_ptr())
+        y, dx = torch.full((n, dout), 77.0, dtype=c.out, device="cuda"), torch.full((n, din), 77.0, dtype=c.out, device="cuda")
+        da, db = torch.empty_like(c.a, dtype=c.out), torch.empty_like(c.b, dtype=c.out)
+        if backward:
+            engine.project_adapted_backward_dev(c.proj, n, c.dy.data_ptr(), dout, c.x.data_ptr(), din, *seg, dx.data_ptr(), din,
+                                                da.data_ptr(), db.data_ptr(), ws, size)
+        else:
+            engine.project_adapted_dev(c.proj, n, c.x.data_ptr(), din, *seg, y.data_ptr(), dout, ws, size)
+        torch.cuda.synchronize()
+        assert bool((buf[:guard] == 255).all()) and bool((buf[guard + size:] == 255).all())
+        if backward:
+            for name, got, (v, m), terms in zip(("dx", "da", "db"), (dx, da, db), want_back, (dout + rank, n + dout, n + din)):
+                close(got, v, m, terms, name)
+        else:
+            close(y, *want, din + rank, "y")
