@@ -269,7 +269,8 @@ int vdb_merge_records_dev(int nparts, int64_t nq, int k, int metric, const void*
  * capture. */
 typedef struct vdb_projection {
     int64_t dim_in, dim_out;     /* 1 .. 65536 */
-    int32_t dtype;               /* VDB_F32, VDB_BF16, VDB_F16: type of rows, of incoming gradients and of every weight */
+    int32_t dtype;               /* VDB_F32, VDB_BF16, VDB_F16: type of rows, of incoming gradients (also where out_dtype is
+                                  * VDB_F32: the caller rounds them) and of every weight */
     int32_t out_dtype;           /* type of what a call writes: dtype, or VDB_F32 */
     int32_t groups;              /* matrices in w, 1 .. 4096; adapted calls take one */
     int32_t adapters;            /* adapters in a, b, scale, up to 65535; 0: none */
@@ -299,7 +300,8 @@ int vdb_project_adapted_dev(const vdb_projection* p, int64_t n, const void* x, i
                             void* workspace, int64_t workspace_bytes, void* stream);
 /* dx = W^T dy + s A^T B^T dy, da [adapters][rank][dim_in] and db [adapters][dim_out][rank] summed over every row that
  * used the adapter (zero for one that none used).  The shared matrix is taken as fixed; its gradient is that of
- * vdb_project_grouped_backward_dev with one group.  dx may be NULL, and da and db together. */
+ * vdb_project_grouped_backward_dev with one group.  dx may be NULL, and da and db together.  Every adapter looks through the ids of all
+ * requests: the cost of da and db grows with adapters times requests. */
 int vdb_project_adapted_backward_dev(const vdb_projection* p, int64_t n, const void* dy, int64_t lddy, const void* x,
                                      int64_t ldx, int64_t requests, const int64_t* offsets, const int32_t* adapter_ids,
                                      void* dx, int64_t lddx, void* da, void* db,

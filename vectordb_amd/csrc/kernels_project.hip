@@ -151,8 +151,8 @@ template <int DT, int NRB, int F> constexpr int pj_shrink_block_lds() {
 // order.  Each adapter that the 16 rows meet is multiplied on its own and keeps its own rows; `share` workgroups divide
 // the adapters of a block of rows among them.  The rows are loaded before the adapters are known.
 // What bounds it is latency (offsets, then the factor, then the exchange): a wave to 16 rows without the exchange, and 64 rows
-// to a workgroup, which reads the factor a quarter as often, were both slower (56 and 45 against 47 us for 32 768 x 1024 rows of
-// rank 64, 24 and 26 against 18 us for 16 384 x 768 of rank 16).
+// to a workgroup, which reads the factor a quarter as often, were both slower at small ranks (24 and 26 against 18 us for
+// 16 384 x 768 of rank 16; for many rows of ranks above 32 see proj_shrink_tile_kernel).
 template <int DT, int NRB, bool XV, int F>
 __device__ __forceinline__ void pj_shrink_block(const ProjShrink& p, long long r0, int mine, int share, char* smem) {
     typedef typename PJ<DT>::T T;
@@ -216,7 +216,7 @@ proj_shrink_pair_kernel(ProjShrink g, ProjShrink h, int share) {
 // Many rows of long requests: 64 rows by all ranks through LDS, a ring of four stages of 128 bytes of k as in PJProduct, each
 // wave 16 rows.  For every adapter of the 64 rows (up to four) the whole product; 64 rows of more adapters are left to the
 // workgroups behind the first `tiles`, which take 16 rows each as above and have nothing to do otherwise.
-// (32 768 x 1024 rows, rank 64: 47 us by 16 rows, which read the factor four times as often.)
+// (32 768 x 1024 rows, rank 64: 29 us, and 52 by 16 rows, which read the factor four times as often.)
 template <int DT, int NRB, int F>
 __global__ void __launch_bounds__(256)
 proj_shrink_tile_kernel(ProjShrink p, int tiles) {
@@ -636,8 +636,8 @@ hipError_t launch_proj_weights_sum(const ProjWeights& p, hipStream_t st) {
     return pj_launch(proj_weights_sum_kernel<VDB_F16>, grid, 0, p, st);
 }
 
-// By 64 rows: from rank 33 and 16 384 rows on, for long requests (rank 64, 1024 wide, 48 requests: 32 768 rows 47 -> 26 us, 8192 rows
-// 22 -> 30; rank 16, 768 wide: 16 384 rows 12 -> 17).
+// By 64 rows: from rank 33 and 16 384 rows on, for long requests (rank 64, 1024 wide, 48 requests: 32 768 rows 52 -> 29 us, 8192 rows
+// 22 -> 33; rank 16, 768 wide: 16 384 rows 12 -> 17).
 template <int DT, int NRB> static bool shrink_tiles(const ProjShrink& p) {
     return NRB >= 4 && p.n >= 16384 && p.n / p.segments >= 128 && proj_shrink_tile_grid(p.n) <= PROJ_MAX_WORKGROUPS;
 }
