@@ -368,3 +368,16 @@ def test_adapted_calls_stay_in_the_workspace(engine, n, din, dout, adapters, ran
                 close(got, v, m, terms, name)
         else:
             close(y, *want, din + rank, "y")
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,din,dout,rank", [(1, 65536, 3, 128), (5, 3, 65536, 17), (40, 65536, 24, 64), (70, 40, 65535, 8), (300, 65536, 8, 16)])
+def test_the_widest_rows(engine, n, din, dout, rank, dtype, out):
+    """65 536 elements in or out, alone and with adapters of the largest rank."""
+    Case(n, din, dout, [0, n // 2, n], dtype, out).check(engine)
+    off = [0, n // 3, n // 2, n]
+    c = Case(n, din, dout, off, dtype, out, 4, rank, [3, -1, 1])
+    if out == "f16":
+        check_in_range(c, engine)
+    else:
+        c.check(engine)

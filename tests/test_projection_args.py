@@ -148,6 +148,14 @@ def test_one_workspace_serves_both_gradients_of_a_handle_with_adapters(n, din, d
         lib.vdb_projection_workspace_bytes(C.byref(struct(dim_in=din, dim_out=dout)), n, 3, 1)
 
 
+def test_an_insert_buffer_is_a_size():
+    """The option divides a projected insert into pieces."""
+    lib = _lib.load()
+    for bad in (0.0, -1.0, float("nan"), float("-inf")):
+        assert lib.vdb_set_option(b"insert_buffer_size_gb", bad) == _lib.EINVAL
+    assert lib.vdb_set_option(b"insert_buffer_size_gb", 1.0) == _lib.OK
+
+
 @pytest.mark.parametrize("fn,n,at", [(fn, 5000, at) for fn in ("adapted", "adapted_backward") for at in (W, A, B, S, OFF, IDS)] +
                          [("grouped_backward", 20000, W), ("grouped_backward", 20000, OFF)])
 @pytest.mark.parametrize("part", ["first", "last"])

@@ -1015,7 +1015,7 @@ int vdb_set_option(const char* key, double value) {
     const std::string k(key);
     if (k == "use_blas_threshold") { if (value < 1) return fail(VDB_EINVAL, "use_blas_threshold < 1"); G.use_blas_threshold = (int)value; }
     else if (k == "cache_capacity_gb") { if (value < 0) return fail(VDB_EINVAL, "cache_capacity_gb < 0"); G.cache_capacity_gb = value; }
-    else if (k == "insert_buffer_size_gb") { if (value <= 0) return fail(VDB_EINVAL, "insert_buffer_size_gb <= 0"); G.insert_buffer_gb = value; }
+    else if (k == "insert_buffer_size_gb") { if (!(value > 0)) return fail(VDB_EINVAL, "insert_buffer_size_gb is not above 0"); G.insert_buffer_gb = value; }
     else if (k == "scan_nt") G.tune_nt = value != 0;
     else if (k == "scan_waves") { if (value < 0 || value > 16) return fail(VDB_EINVAL, "scan_waves not in [0,16]"); G.tune_waves = (int)value; }
     else if (k == "scan_blocks_per_cu") { if (value < 0 || value > 32) return fail(VDB_EINVAL, "scan_blocks_per_cu not in [0,32]"); G.tune_bpc = (int)value; }
@@ -2388,7 +2388,7 @@ int vdb_insert_projected_dev(const char* name, const vdb_projection* p, int64_t 
         // The rows are projected and appended in pieces of the insert buffer's size, through memory that stays with a workspace:
         // hipFree would wait for every search in flight.  All of them are published at once.
         const double fit = G.insert_buffer_gb * 1073741824.0 / ((double)t->dim * sizeof(float));
-        const int64_t most = fit < 1 ? 1 : fit > (double)n ? n : (int64_t)fit;
+        const int64_t most = !(fit >= 1) ? 1 : fit > (double)n ? n : (int64_t)fit;
         const int64_t pieces = (n + most - 1) / most, piece = (n + pieces - 1) / pieces;
         const size_t rb = round_up((size_t)piece * t->dim * sizeof(float), 256);
         HeldWorkspace held(st);
