@@ -381,3 +381,65 @@ def test_the_widest_rows(engine, n, din, dout, rank, dtype, out):
         check_in_range(c, engine)
     else:
         c.check(engine)
+
+
+def test_projected_inserts_and_searches_at_once(engine, table_name):
+    """Host threads with streams of their own: three search one table through different projections, two insert into others."""
+    import threading
+    dim, n, k = 96, 5000, 5
+    engine.create_table(table_name, dim, _lib.METRIC_L2, _lib.F32)
+    rows = torch.randn(n, dim, generator=torch.Generator().manual_seed(3)).cuda()
+    ids = torch.arange(n, dtype=torch.int64, device="cuda")
+    engine.insert_dev(table_name, n, rows.data_ptr(), ids.data_ptr())
+    queries = [Case(30 + 100 * i, 64 + 8 * i, dim, [0, 10, 11, 30 + 100 * i], d, "f32", 3, 8 + 4 * i, [2, -1, 0], seed=i)
+               for i, d in enumerate(("bf16", "f32", "f16"))]
+    sources = [Case(2000 + 500 * i, 72, dim, [0, 600, 2000 + 500 * i], "bf16", "f32", seed=9 + i) for i in range(2)]
+    others = [table_name + "_a", table_name + "_b"]
+    for o in others:
+        engine.create_table(o, dim, _lib.METRIC_L2, _lib.F32)
+
+    def search(c, stream):
+        out = (torch.full((c.n, k), -5, dtype=torch.int64, device="cuda"), torch.zeros(c.n, k, device="cuda"),
+               torch.zeros(c.n, dtype=torch.int32, device="cuda"))
+        engine.search_projected_dev(table_name, c.proj, c.n, c.x.data_ptr(), c.din, 3, c.offsets.data_ptr(), c.ids_dev.data_ptr(), k,
+                                    *(t.data_ptr() for t in out), stream=stream)
+        return out
+    try:
+        want = [search(c, 0) for c in queries]
+        torch.cuda.synchronize()
+        errors = []
+
+        def searcher(i):
+            try:
+                stream = torch.cuda.Stream()
+                with torch.cuda.stream(stream):
+                    for _ in range(20):
+                        got = search(queries[i], stream.cuda_stream)
+                        stream.synchronize()
+                        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+            except BaseException as exc:                          # noqa: BLE001 (reported below)
+                errors.append(exc)
+
+        def inserter(i):
+            try:
+                stream, c = torch.cuda.Stream(), sources[i]
+                for _ in range(10):
+                    engine.insert_projected_dev(others[i], c.proj, c.n, c.x.data_ptr(), c.din, c.offsets.data_ptr(), ids.data_ptr(),
+                                                stream=stream.cuda_stream)
+            except BaseException as exc:                          # noqa: BLE001
+                errors.append(exc)
+        threads = [threading.Thread(target=searcher, args=(i,)) for i in range(3)] + [threading.Thread(target=inserter, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors, errors[0]
+        for o, c in zip(others, sources):
+            assert engine.count(o) == 10 * c.n
+            stored, _ = engine.fetch_rows(o, 0, 10 * c.n)
+            want_rows, mag = c.want_forward()
+            for i in range(10):
+                close(torch.from_numpy(stored[i * c.n:(i + 1) * c.n]), want_rows, mag, 72, "rows")
+    finally:
+        for o in others:
+            engine.drop_table(o)
